@@ -394,8 +394,10 @@ def _plain_step(s):
     cos, sin = s["cos"][pos], s["sin"][pos]  # (B, N, D / 2)
     k = _plain_rotate(s["k_new"].view(B, N, Hk, D), cos.unsqueeze(2), sin.unsqueeze(2))
     at = _plain_slots(s, base.unsqueeze(1) + node)
-    s["k"].view(-1, Hk, D)[at] = k
-    s["v"].view(-1, Hk, D)[at] = s["v_new"].view(B, N, Hk, D)
+    pool_k, pool_v = s["k"].view(-1, Hk, D), s["v"].view(-1, Hk, D)
+    node_row = real.view(B, N, 1, 1)  # a padding slot's rows stay as they are
+    pool_k[at] = torch.where(node_row, k, pool_k[at])
+    pool_v[at] = torch.where(node_row, s["v_new"].view(B, N, Hk, D), pool_v[at])
     q = _plain_rotate(s["q"], cos.unsqueeze(1), sin.unsqueeze(1))
     return _plain_attend({**s, "q": q}, seen), s["k"], s["v"]
 
@@ -586,8 +588,10 @@ def exact(c, seed):
             d = h + torch.tensor(depth, device=DEV)
             cos, sin = s["cos"][d].double(), s["sin"][d].double()
             q = _exact_rotate(q, cos, sin)
-            kp[at[h:]] = _exact_rotate(s["k_new"][b * N:(b + 1) * N], cos.unsqueeze(1), sin.unsqueeze(1))
-            vp[at[h:]] = s["v_new"][b * N:(b + 1) * N]
+            n = sum(p >= -1 for p in lists[b])  # a padding slot's rows stay as they are
+            new = slice(b * N, b * N + n)
+            kp[at[h:h + n]] = _exact_rotate(s["k_new"][new], cos[:n].unsqueeze(1), sin[:n].unsqueeze(1))
+            vp[at[h:h + n]] = s["v_new"][new]
         outs.append(_exact_attend(q.double(), kp[at].double(), vp[at].double(), see.to(DEV)))
     o = torch.stack(outs)
     return o if c["kind"] == "attend" else (o, s["k"].double(), s["v"].double())
