@@ -27,8 +27,8 @@ TIMELINE_LIB_PATH = os.path.join(PKG_DIR, "libcie_attn_timeline.so")
 # stand-alone microbenchmarks (benchmarks/<name>.hip -> _build/<name>), not part of the library
 BENCH_TOOLS = ("vector_rates", "read_floor", "prefill_step")
 
-SOURCES = ["capi.cpp", "paged_plan.cpp", "flash_fwd.hip", "paged_fwd.hip", "kv_append.hip", "rope.hip",
-           "int8_gemm.hip"]
+SOURCES = ["capi.cpp", "paged_plan.cpp", "flash_fwd.hip", "paged_fwd.hip", "tree_fwd.hip", "draft.hip",
+           "kv_append.hip", "rope.hip", "int8_gemm.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 COMMON = [

@@ -965,3 +965,251 @@ int cie_rope_apply(const void* x, void* out, const int64_t* x_stride, const int6
 }
 
 }  // extern "C"
+
+static cie::TreeGeom tree_geom(int B, int Hq, int Hk, int N, int D, int ctx_limit, int block_size) {
+  return cie::tree_geometry(B, Hq, Hk, N, D, ctx_limit, block_size, cie::device_shape());
+}
+
+extern "C" {
+
+size_t cie_tree_workspace_bytes(int B, int Hq, int Hk, int N, int D, int max_context, int block_size,
+                                int max_blocks_per_seq) {
+  if (block_size < 1 || max_blocks_per_seq < 0 || (int64_t)max_blocks_per_seq * block_size > 0x7fffffff || Hk < 1) return 0;
+  const cie::TreeGeom g =
+      tree_geom(B, Hq, Hk, N, D, paged_ctx_limit(max_context, block_size, max_blocks_per_seq), block_size);
+  return g.ok ? g.info_bytes + g.ml_bytes + g.part_bytes : 0;
+}
+
+int cie_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                  const int32_t* block_tables, const int32_t* context_lens, const int32_t* tree_mask,
+                  const int32_t* depths, void* o, void* workspace, size_t workspace_bytes,
+                  const int64_t* q_stride, const int64_t* kn_stride, const int64_t* vn_stride,
+                  const int64_t* kc_stride, const int64_t* vc_stride, const int64_t* o_stride,
+                  int64_t mask_batch_stride, int64_t depths_batch_stride, int B, int Hq, int Hk, int N, int D,
+                  int num_blocks, int block_size, int max_blocks_per_seq, int max_context, float scale, int dtype,
+                  const void* rope_cos, const void* rope_sin, int rope_rows, int rope_dtype, void* stream) {
+  CIE_TRY(common_checks(Hq, Hk, D, dtype));
+  if (B < 0 || N < 0) return fail(CIE_EINVAL, "negative size (B=%d, N=%d)", B, N);
+  if (block_size < 1) return fail(CIE_EINVAL, "block_size must be positive, got %d", block_size);
+  if (num_blocks < 0 || max_blocks_per_seq < 0)
+    return fail(CIE_EINVAL, "negative pool geometry (num_blocks=%d, max_blocks_per_seq=%d)", num_blocks,
+                max_blocks_per_seq);
+  if ((int64_t)max_blocks_per_seq * block_size > 0x7fffffff)
+    return fail(CIE_EINVAL, "max_blocks_per_seq * block_size exceeds 2^31");
+  if (!std::isfinite(scale)) return fail(CIE_EINVAL, "scale must be finite");
+  if ((int64_t)B * N == 0) {
+    g_err.clear();
+    return CIE_OK;
+  }
+  CIE_TRY(check_ptr("q", q));
+  CIE_TRY(check_ptr("o", o));
+  CIE_TRY(check_ptr("k_cache", k_cache));
+  CIE_TRY(check_ptr("v_cache", v_cache));
+  if (!block_tables || !context_lens || !tree_mask)
+    return fail(CIE_EINVAL, "block_tables / context_lens / tree_mask: NULL pointer");
+  CIE_TRY(check_strides("q", q_stride));
+  CIE_TRY(check_strides("o", o_stride));
+  CIE_TRY(check_strides("k_cache", kc_stride));
+  CIE_TRY(check_strides("v_cache", vc_stride));
+  if ((int64_t)(Hk - 1) * std::max(kc_stride[2], vc_stride[2]) + D >= ((int64_t)1 << 31))
+    return fail(CIE_EINVAL, "k_cache / v_cache: the kv heads of a token span 2^31 elements or more");
+  if (mask_batch_stride < 0 || depths_batch_stride < 0) return fail(CIE_EINVAL, "tree_mask / depths: negative stride");
+  if (rope_cos || rope_sin) {
+    CIE_TRY(check_rope(rope_cos, rope_sin, rope_rows, rope_dtype));
+    if (!depths) return fail(CIE_EINVAL, "rope needs the nodes' depths");
+  }
+  if (k_new || v_new) {
+    CIE_TRY(check_ptr("k_new", k_new));
+    CIE_TRY(check_ptr("v_new", v_new));
+    if (!kn_stride || !vn_stride) return fail(CIE_EINVAL, "k_new / v_new strides: NULL pointer");
+    for (int i = 0; i < 2; ++i)
+      if (kn_stride[i] < 0 || kn_stride[i] % 8 || vn_stride[i] < 0 || vn_stride[i] % 8)
+        return fail(CIE_EINVAL, "k_new / v_new strides must be non-negative multiples of 8 elements");
+  }
+  const int ctx_limit = paged_ctx_limit(max_context, block_size, max_blocks_per_seq);
+  if ((int64_t)B * ((ctx_limit + 31) / 32) > 0x7fffffff) return fail(CIE_EINVAL, "problem too large for one launch");
+  const cie::TreeGeom g = tree_geom(B, Hq, Hk, N, D, ctx_limit, block_size);
+  if (!g.ok) return fail(CIE_EINVAL, "tree attention: %s", g.err);
+  const size_t need = g.info_bytes + g.ml_bytes + g.part_bytes;
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail(CIE_EWORKSPACE, "workspace of %zu bytes required, %zu given", need,
+                  workspace ? workspace_bytes : (size_t)0);
+    if (!aligned16(workspace)) return fail(CIE_EINVAL, "workspace: pointer is not 16-byte aligned");
+  }
+  cie::TreeParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.kc = static_cast<const uint16_t*>(k_cache);
+  p.vc = static_cast<const uint16_t*>(v_cache);
+  p.o = static_cast<uint16_t*>(o);
+  p.bt = block_tables;
+  p.lens = context_lens;
+  p.mask = tree_mask;
+  p.depths = depths;
+  if (need > 0) {
+    char* const ws = static_cast<char*>(workspace);
+    p.info = reinterpret_cast<int2*>(ws);
+    p.ml = reinterpret_cast<float2*>(ws + g.info_bytes);
+    p.part = reinterpret_cast<float*>(ws + g.info_bytes + g.ml_bytes);
+  }
+  p.qs0 = q_stride[0]; p.qs1 = q_stride[1]; p.qs2 = q_stride[2];
+  p.ks0 = kc_stride[0]; p.ks1 = kc_stride[1]; p.ks2 = kc_stride[2];
+  p.vs0 = vc_stride[0]; p.vs1 = vc_stride[1]; p.vs2 = vc_stride[2];
+  p.os0 = o_stride[0]; p.os1 = o_stride[1]; p.os2 = o_stride[2];
+  p.W = (N + 31) / 32;
+  p.ms0 = mask_batch_stride; p.ms1 = p.W; p.ds0 = depths_batch_stride;
+  p.B = B; p.Hk = Hk; p.N = N; p.group = Hq / Hk; p.R = g.R; p.D = D;
+  p.num_blocks = num_blocks; p.max_blocks = max_blocks_per_seq; p.block_size = block_size; p.ctx_limit = ctx_limit;
+  p.bsdiv = cie::make_fastdiv((uint32_t)block_size);
+  p.ndiv = cie::make_fastdiv((uint32_t)N);
+  p.updiv = cie::make_fastdiv((uint32_t)(Hk * D / 16));
+  p.HG = g.HG; p.NG = g.NG; p.NRT = g.NRT; p.NCH = g.NCH; p.NST = g.NST;
+  p.extra = g.extra; p.cmin = g.cmin;
+  p.xcd_shift = cie::device_shape().xcd_shift;
+  set_scale(scale, &p.scale_log2, &p.q_sign);
+  if (rope_cos) p.rope = cie::RopeTables{rope_cos, rope_sin, rope_rows, rope_dtype};
+  if (k_new) {
+    p.kn = static_cast<const uint16_t*>(k_new);
+    p.vn = static_cast<const uint16_t*>(v_new);
+    p.kns0 = kn_stride[0]; p.kns1 = kn_stride[1];
+    p.vns0 = vn_stride[0]; p.vns1 = vn_stride[1];
+  }
+  return launch_status(cie::launch_tree(p, g, dtype, D, static_cast<hipStream_t>(stream)));
+}
+
+int cie_draft_masks(const int32_t* parents, int32_t* mask, int32_t* depths, uint32_t* status, int B, int N,
+                    void* stream) {
+  if (B < 0 || N < 0) return fail(CIE_EINVAL, "negative size (B=%d, N=%d)", B, N);
+  if (N > cie::kTreeMaxNodes) return fail(CIE_EINVAL, "a draft tree has at most %d nodes, got %d", cie::kTreeMaxNodes, N);
+  if ((int64_t)B * N == 0) {
+    g_err.clear();
+    return CIE_OK;
+  }
+  if (!parents || !mask || !depths) return fail(CIE_EINVAL, "parents / mask / depths: NULL pointer");
+  return launch_status(cie::launch_draft_masks(parents, mask, depths, status, B, N, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"
+
+static int verify_impl(const void* target, const void* draft, const void* draft_tokens, int token_bytes,
+                       const int32_t* parents, const void* uniforms, int uniform_bytes, void* tokens, int32_t* path,
+                       int32_t* counts, const int64_t* ts, const int64_t* ds, int B, int N, int V, int dtype, int mode,
+                       void* stream) {
+  if (dtype != CIE_TABLE_F16 && dtype != CIE_TABLE_BF16 && dtype != CIE_TABLE_F32)
+    return fail(CIE_EDTYPE, "unsupported dtype code %d (f16 = 0, bf16 = 1, f32 = 2)", dtype);
+  if (B < 0 || N < 0 || V < 0) return fail(CIE_EINVAL, "negative size (B=%d, N=%d, V=%d)", B, N, V);
+  if (N > cie::kTreeMaxNodes) return fail(CIE_EINVAL, "a draft tree has at most %d nodes, got %d", cie::kTreeMaxNodes, N);
+  if (V > (1 << 30)) return fail(CIE_EINVAL, "vocabulary of %d entries, at most 2^30", V);
+  if ((int64_t)B * N == 0) {
+    g_err.clear();
+    return CIE_OK;
+  }
+  if (V < 1) return fail(CIE_EINVAL, "the vocabulary is empty");
+  if (token_bytes != 4 && token_bytes != 8) return fail(CIE_EINVAL, "tokens of %d bytes, expected 4 or 8", token_bytes);
+  if (!target || !draft_tokens || !parents || !tokens || !path || !counts || !ts)
+    return fail(CIE_EINVAL, "verification: NULL pointer");
+  const uintptr_t elt = dtype == CIE_TABLE_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(target) & elt) || (reinterpret_cast<uintptr_t>(draft) & elt))
+    return fail(CIE_EINVAL, "probabilities: pointer not aligned to their type");
+  if (mode >= 0) {
+    if (!uniforms || (uniform_bytes != 4 && uniform_bytes != 8))
+      return fail(CIE_EINVAL, "uniforms: NULL pointer or %d bytes each, expected 4 or 8", uniform_bytes);
+    if (mode > 0 && !ds) return fail(CIE_EINVAL, "draft probabilities: stride array is NULL");
+  }
+  if (ts[0] < 0 || ts[1] < 0 || (mode > 0 && (ds[0] < 0 || ds[1] < 0)))
+    return fail(CIE_EINVAL, "probabilities: negative stride");
+  cie::VerifyParams p{};
+  p.target = target;
+  p.draft = draft;
+  p.draft_tokens = draft_tokens;
+  p.parents = parents;
+  p.uniforms = uniforms;
+  p.tokens = tokens;
+  p.path = path;
+  p.counts = counts;
+  p.ts0 = ts[0]; p.ts1 = ts[1];
+  if (mode > 0) p.ds0 = ds[0], p.ds1 = ds[1];
+  p.token_bytes = token_bytes;
+  p.uniform_bytes = uniform_bytes;
+  p.B = B; p.N = N; p.V = V;
+  return launch_status(cie::launch_verify(p, mode, dtype, static_cast<hipStream_t>(stream)));
+}
+
+extern "C" {
+
+int cie_verify_draft(const void* target_probs, const void* draft_probs, const void* draft_tokens, int token_bytes,
+                     const int32_t* parents, const void* uniforms, int uniform_bytes, void* tokens, int32_t* path,
+                     int32_t* counts, const int64_t* target_stride, const int64_t* draft_stride, int B, int N, int V,
+                     int dtype, int replacement, void* stream) {
+  return verify_impl(target_probs, draft_probs, draft_tokens, token_bytes, parents, uniforms, uniform_bytes, tokens,
+                     path, counts, target_stride, draft_stride, B, N, V, dtype,
+                     !draft_probs ? 0 : replacement ? 1 : 2, stream);
+}
+
+int cie_verify_greedy(const void* target_logits, const void* draft_tokens, int token_bytes, const int32_t* parents,
+                      void* tokens, int32_t* path, int32_t* counts, const int64_t* target_stride, int B, int N, int V,
+                      int dtype, void* stream) {
+  return verify_impl(target_logits, nullptr, draft_tokens, token_bytes, parents, nullptr, 0, tokens, path, counts,
+                     target_stride, nullptr, B, N, V, dtype, -1, stream);
+}
+
+int cie_kv_keep(void* const* k_caches, void* const* v_caches, int layers, const int64_t* k_stride,
+                const int64_t* v_stride, const int32_t* block_tables, const int32_t* starts, const int32_t* path,
+                int64_t path_stride, const int32_t* counts, int B, int N, int heads, int64_t head_bytes,
+                int num_blocks, int block_size, int max_blocks_per_seq, void* stream) {
+  if (layers < 0 || B < 0 || N < 0) return fail(CIE_EINVAL, "negative size (layers=%d, B=%d, N=%d)", layers, B, N);
+  if (N > cie::kTreeMaxNodes) return fail(CIE_EINVAL, "a draft tree has at most %d nodes, got %d", cie::kTreeMaxNodes, N);
+  if (heads < 1 || head_bytes < 16 || head_bytes % 16 || head_bytes > 4096)
+    return fail(CIE_EINVAL, "head rows must be multiples of 16 bytes up to 4096, got %lld x %d", (long long)head_bytes, heads);
+  if (block_size < 1 || num_blocks < 0 || max_blocks_per_seq < 0)
+    return fail(CIE_EINVAL, "invalid pool geometry (num_blocks=%d, block_size=%d, max_blocks_per_seq=%d)", num_blocks,
+                block_size, max_blocks_per_seq);
+  if ((int64_t)max_blocks_per_seq * block_size > 0x7fffffff)
+    return fail(CIE_EINVAL, "max_blocks_per_seq * block_size exceeds 2^31");
+  const int64_t chunks = head_bytes / 16 * heads;
+  if (2 * chunks * cie::kKeepLayers >= ((int64_t)1 << 31) || B > 65535)
+    return fail(CIE_EINVAL, "problem too large for one launch");
+  if (layers == 0 || (int64_t)B * N == 0) {
+    g_err.clear();
+    return CIE_OK;
+  }
+  if (!k_caches || !v_caches || !k_stride || !v_stride || !block_tables || !starts || !path || !counts)
+    return fail(CIE_EINVAL, "kv_keep: NULL pointer");
+  if (path_stride < 0) return fail(CIE_EINVAL, "path: negative stride");
+  for (int i = 0; i < 3; ++i)
+    if (k_stride[i] < 0 || k_stride[i] % 16 || v_stride[i] < 0 || v_stride[i] % 16)
+      return fail(CIE_EINVAL, "pool strides must be non-negative multiples of 16 bytes");
+  for (int l = 0; l < layers; ++l) {
+    CIE_TRY(check_ptr("k_caches", k_caches[l]));
+    CIE_TRY(check_ptr("v_caches", v_caches[l]));
+  }
+  cie::KeepParams p{};
+  p.bt = block_tables;
+  p.starts = starts;
+  p.path = path;
+  p.counts = counts;
+  p.ps0 = path_stride;
+  for (int x = 0; x < 2; ++x) {
+    const int64_t* s = x ? v_stride : k_stride;
+    p.block[x] = s[0], p.token[x] = s[1], p.head[x] = s[2];
+  }
+  p.N = N;
+  p.max_blocks = max_blocks_per_seq; p.num_blocks = num_blocks; p.block_size = block_size;
+  p.cpr = (uint32_t)chunks;
+  p.cph = (uint32_t)(head_bytes / 16);
+  p.cprdiv = cie::make_fastdiv(p.cpr);
+  p.cphdiv = cie::make_fastdiv(p.cph);
+  p.bsdiv = cie::make_fastdiv((uint32_t)block_size);
+  for (int l0 = 0; l0 < layers; l0 += cie::kKeepLayers) {
+    p.layers = std::min(cie::kKeepLayers, layers - l0);
+    for (int l = 0; l < p.layers; ++l) {
+      p.pools[2 * l] = static_cast<char*>(k_caches[l0 + l]);
+      p.pools[2 * l + 1] = static_cast<char*>(v_caches[l0 + l]);
+    }
+    const hipError_t e = cie::launch_kv_keep(p, B, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return launch_status(e);
+  }
+  return launch_status(hipSuccess);
+}
+
+}  // extern "C"

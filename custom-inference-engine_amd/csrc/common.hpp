@@ -319,6 +319,71 @@ __device__ __forceinline__ int chunk_swizzle(int r) {
   else return (r >> 3) & 1;
 }
 
+// Swizzle of the 16-byte chunks of token row t in a tile with nch chunks per
+// row: the family of chunk_swizzle applied to rows of nch chunks.
+__device__ __forceinline__ int row_swizzle(int nch, int t) {
+  return nch >= 16 ? bitrev4(t & 15) : nch == 8 ? bitrev3((t >> 1) & 7) : nch == 4 ? ((t >> 2) & 3) : ((t >> 3) & 1);
+}
+
+// Inclusive prefix sum over the 64 lanes: DPP row shifts within each row of
+// 16 lanes, then the row totals broadcast forward (row_bcast:15 into rows 1
+// and 3, row_bcast:31 into rows 2 and 3). Lanes whose DPP source lies
+// outside the row, and rows outside the row mask, add the old value 0.
+__device__ __forceinline__ int wave_incl_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+
+// Combines two partial softmax states (running maximum, sum, four output columns).
+__device__ __forceinline__ void merge_state(float& M, float& L, float4& A, float m2, float l2, float4 a2) {
+  const float Mn = maxf(M, m2);
+  const float wo = rescale_weight(M, Mn), wn = rescale_weight(m2, Mn);
+  L = L * wo + l2 * wn;
+  A.x = A.x * wo + a2.x * wn;
+  A.y = A.y * wo + a2.y * wn;
+  A.z = A.z * wo + a2.z * wn;
+  A.w = A.w * wo + a2.w * wn;
+  M = Mn;
+}
+
+// Value of lane (lane ^ OFF) for OFF = 1, 2, 4, by DPP: quad permutations for
+// 1 and 2, the two row rotations by 4 (row_ror:12 reads lane + 4, row_ror:4
+// reads lane - 4 within each row of 16) for 4.
+template <int OFF>
+__device__ __forceinline__ float lane_xor(float x) {
+  const int v = __float_as_int(x);
+  if constexpr (OFF == 1) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, false));  // quad_perm [1,0,3,2]
+  } else if constexpr (OFF == 2) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, false));  // quad_perm [2,3,0,1]
+  } else {
+    static_assert(OFF == 4, "lane_xor: 1, 2 or 4");
+    const int up = __builtin_amdgcn_mov_dpp(v, 0x12c, 0xf, 0xf, false);  // row_ror:12
+    const int dn = __builtin_amdgcn_mov_dpp(v, 0x124, 0xf, 0xf, false);  // row_ror:4
+    return __int_as_float((threadIdx.x & 4) ? dn : up);
+  }
+}
+
+template <int OFF>
+__device__ __forceinline__ void butterfly_step(int t, float& M, float& L, float4& A) {
+  const float m2 = lane_xor<OFF>(M), l2 = lane_xor<OFF>(L);
+  const float4 a2 = {lane_xor<OFF>(A.x), lane_xor<OFF>(A.y), lane_xor<OFF>(A.z), lane_xor<OFF>(A.w)};
+  // the lower lane of each pair keeps its own state first: same order in both lanes
+  if (t & OFF) {
+    float Mx = m2, Lx = l2;
+    float4 Ax = a2;
+    merge_state(Mx, Lx, Ax, M, L, A);
+    M = Mx, L = Lx, A = Ax;
+  } else {
+    merge_state(M, L, A, m2, l2, a2);
+  }
+}
+
 // Transpose helpers for 16-bit data held two per dword: from four rows
 // r0..r3 (dword w covers columns 2w, 2w+1) build the 4 keys of column 2w
 // (even) or 2w+1 (odd) as an 8-byte [r0 r1 r2 r3] pair of dwords.

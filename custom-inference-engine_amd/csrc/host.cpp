@@ -47,10 +47,18 @@ struct Api {
   decltype(&cie_kv_gather) gather;
   decltype(&cie_int8_matmul_workspace_bytes) int8_ws;
   decltype(&cie_int8_matmul) int8;
+  decltype(&cie_draft_masks) masks;
+  decltype(&cie_tree_workspace_bytes) tree_ws;
+  decltype(&cie_tree_attn) tree;
+  decltype(&cie_verify_draft) verify;
+  decltype(&cie_verify_greedy) greedy;
+  decltype(&cie_kv_keep) keep;
 } api;
 const char* const kNames[] = {"cie_flash_workspace_bytes", "cie_flash_fwd_ex", "cie_flash_paged_workspace_bytes",
                               "cie_flash_paged", "cie_paged_workspace_bytes", "cie_paged_fwd_ex", "cie_kv_append",
-                              "cie_kv_append_rope", "cie_kv_append_seq", "cie_kv_gather", "cie_int8_matmul_workspace_bytes", "cie_int8_matmul"};
+                              "cie_kv_append_rope", "cie_kv_append_seq", "cie_kv_gather", "cie_int8_matmul_workspace_bytes", "cie_int8_matmul",
+                              "cie_draft_masks", "cie_tree_workspace_bytes", "cie_tree_attn", "cie_verify_draft",
+                              "cie_verify_greedy", "cie_kv_keep"};
 constexpr size_t kFns = sizeof(kNames) / sizeof(kNames[0]);
 static_assert(sizeof(Api) == kFns * sizeof(void*), "one name per function, in order");
 
@@ -576,6 +584,182 @@ PyObject* int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// masks(parents, status | None): (mask, depths, parents as int32)
+PyObject* masks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2) Py_RETURN_NONE;
+  const Tensor* p = tensor(a[0]);
+  bool ok = p != nullptr;
+  const Tensor* status = tensor_or_none(a[1], &ok);
+  if (!ok || !index_ok(p, *p) || p->dim() < 1 || p->dim() > 2 || p->size(-1) > 1024 || !fits(p->size(0))) Py_RETURN_NONE;
+  if (status && (!on_gpu(*status) || status->device() != p->device() || status->numel() < 1 ||
+                 (status->scalar_type() != at::kInt && status->scalar_type() != at::kUInt32)))
+    Py_RETURN_NONE;
+  const c10::OptionalDeviceGuard guard(p->device());
+  const Tensor par = index32(*p);
+  const int64_t N = par.size(-1), B = par.dim() == 2 ? par.size(0) : 1;
+  at::DimVector shape(par.sizes().begin(), par.sizes().end());
+  const Tensor depths = at::empty(shape, par.options());
+  shape.push_back((N + 31) / 32);
+  const Tensor mask = at::empty(shape, par.options());
+  void* stream = stream_of(par);
+  const int rc = launch([&] {
+    return api.masks(ip(par), static_cast<int32_t*>(mask.data_ptr()), static_cast<int32_t*>(depths.data_ptr()),
+                     status ? static_cast<uint32_t*>(status->data_ptr()) : nullptr, (int)B, (int)N, stream);
+  });
+  if (rc) return PyLong_FromLong(rc);
+  PyObject *pm = THPVariable_Wrap(mask), *pd = THPVariable_Wrap(depths), *pp = THPVariable_Wrap(par);
+  return pm && pd && pp ? Py_BuildValue("(NNN)", pm, pd, pp) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// tree(q, k_cache, v_cache, block_tables, context_lens, tree_mask, scale | None, max_context, cos, sin, depths | None,
+// out | None, k_new | None, v_new | None)
+PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 14) Py_RETURN_NONE;
+  const Tensor *q = tensor(a[0]), *m = tensor(a[5]);
+  bool ok = q && m;
+  const Tensor* depths = tensor_or_none(a[10], &ok);
+  const Tensor* o = tensor_or_none(a[11], &ok);
+  const Tensor* kn = tensor_or_none(a[12], &ok);
+  const Tensor* vn = tensor_or_none(a[13], &ok);
+  if (!ok || !on_gpu(*q) || q->dim() != 4 || dtype_code(*q) < 0 || !head_dim_ok(q->size(3))) Py_RETURN_NONE;
+  const int64_t B = q->size(0), Hq = q->size(1), N = q->size(2), D = q->size(3), W = (N + 31) / 32;
+  const Pools P(a[1], a[2], a[3], a[4], *q, B, D);
+  const int64_t mc = PyLong_Check(a[7]) ? PyLong_AsLongLong(a[7]) : -1;
+  if (!P.ok || Hq % P.Hk || !fits(mc) || !fits(B) || !fits(Hq) || !fits(N) || B * Hq * N == 0) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (!on_gpu(*m) || m->device() != q->device() || m->scalar_type() != at::kInt || m->dim() < 2 || m->dim() > 3 ||
+      m->size(-1) != W || m->size(-2) != N || (m->dim() == 3 && m->size(0) != B) || (W > 1 && m->stride(-1) != 1) ||
+      (N > 1 && m->stride(-2) != W))
+    Py_RETURN_NONE;
+  if (o && (!on_gpu(*o) || o->sizes() != q->sizes() || o->scalar_type() != q->scalar_type() ||
+            o->device() != q->device() || !kernel_layout(*o)))
+    Py_RETURN_NONE;
+  const Rope rope(a[8], a[9], D, *q);
+  if (!rope.ok || (depths == nullptr) != (rope.cos == nullptr)) Py_RETURN_NONE;
+  if (depths && (!on_gpu(*depths) || depths->device() != q->device() || depths->scalar_type() != at::kInt ||
+                 depths->dim() < 1 || depths->dim() > 2 || depths->size(-1) != N ||
+                 (depths->dim() == 2 && depths->size(0) != B) || (N > 1 && depths->stride(-1) != 1)))
+    Py_RETURN_NONE;
+  if ((kn == nullptr) != (vn == nullptr)) Py_RETURN_NONE;
+  if (kn)
+    for (const Tensor* t : {kn, vn})
+      if (!on_gpu(*t) || t->device() != q->device() || t->scalar_type() != q->scalar_type() || t->dim() != 3 ||
+          t->size(0) != B * N || t->size(1) != P.Hk || t->size(2) != D)
+        Py_RETURN_NONE;
+  double scale = 1.0 / std::sqrt((double)D);
+  if (a[6] != Py_None && !number(a[6], &scale)) Py_RETURN_NONE;
+  const c10::OptionalDeviceGuard guard(q->device());
+  const Tensor out = o ? *o : at::empty({B, Hq, N, D}, q->options());
+  const size_t nbytes = api.tree_ws((int)B, (int)Hq, (int)P.Hk, (int)N, (int)D, (int)mc, (int)P.block_size, (int)P.width);
+  const Tensor ws = nbytes ? bytes_like(nbytes, *q) : Tensor();
+  const Tensor qc = laid_out(*q), bt = index32(*P.bt), lens = index32(*P.lens);
+  const Tensor kc = kn ? laid_out(*kn) : Tensor(), vc = kn ? laid_out(*vn) : Tensor();
+  const Strides sq(qc), sk(*P.kc), sv(*P.vc), so(out), skn(kn ? kc : qc), svn(kn ? vc : qc);
+  void* stream = stream_of(*q);
+  const int rc = launch([&] {
+    return api.tree(qc.data_ptr(), kn ? kc.data_ptr() : nullptr, kn ? vc.data_ptr() : nullptr, P.kc->data_ptr(),
+                    P.vc->data_ptr(), ip(bt), ip(lens), ip(*m), depths ? ip(*depths) : nullptr, out.data_ptr(),
+                    nbytes ? ws.data_ptr() : nullptr, nbytes, sq.s, skn.s, svn.s, sk.s, sv.s, so.s,
+                    m->dim() == 3 && B > 1 ? m->stride(0) : 0,
+                    depths && depths->dim() == 2 && B > 1 ? depths->stride(0) : 0, (int)B, (int)Hq, (int)P.Hk, (int)N,
+                    (int)D, (int)P.num_blocks, (int)P.block_size, (int)P.width, (int)mc, (float)scale, dtype_code(*q),
+                    rope.cos, rope.sin, rope.rows, rope.dt, stream);
+  });
+  return result(rc, out);
+  END_HANDLE_TH_ERRORS
+}
+
+// verify(target, draft_tokens, parents, uniforms | None, draft | None, replacement): (tokens, path, counts); without
+// uniforms the greedy one
+PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) Py_RETURN_NONE;
+  const Tensor *t = tensor(a[0]), *x = tensor(a[1]), *p = tensor(a[2]);
+  bool ok = t && x && p;
+  const Tensor* u = tensor_or_none(a[3], &ok);
+  const Tensor* d = tensor_or_none(a[4], &ok);
+  if (!ok || !on_gpu(*t) || t->dim() != 3 || any_code(*t) < 0 || !index_ok(x, *t) || !index_ok(p, *t) || (d && !u))
+    Py_RETURN_NONE;
+  const int64_t B = t->size(0), N = t->size(1), V = t->size(2);
+  if (N > 1024 || V < 1 || !fits(B) || !fits(V) || t->stride(2) != 1 || x->dim() != 2 || x->size(0) != B ||
+      x->size(1) != N || p->dim() != 2 || p->size(0) != B || p->size(1) != N)
+    Py_RETURN_NONE;
+  if (u && (!on_gpu(*u) || u->device() != t->device() || u->sizes() != x->sizes() ||
+            (u->scalar_type() != at::kFloat && u->scalar_type() != at::kDouble)))
+    Py_RETURN_NONE;
+  if (d && (!on_gpu(*d) || d->device() != t->device() || d->sizes() != t->sizes() ||
+            d->scalar_type() != t->scalar_type() || d->stride(2) != 1))
+    Py_RETURN_NONE;
+  const int replacement = PyObject_IsTrue(a[5]);
+  if (replacement < 0) return nullptr;
+  const c10::OptionalDeviceGuard guard(t->device());
+  const Tensor xc = x->contiguous(), pc = index32(*p), uc = u ? u->contiguous() : Tensor();
+  const Tensor tokens = at::empty({B, N}, xc.options()), path = at::empty({B, N}, pc.options()),
+               counts = at::empty({B}, pc.options());
+  const Strides st(*t), sd(d ? *d : *t);
+  const int tb = (int)xc.element_size();
+  int32_t *const pp = static_cast<int32_t*>(path.data_ptr()), *const cp = static_cast<int32_t*>(counts.data_ptr());
+  void* stream = stream_of(*t);
+  const int rc = launch([&] {
+    if (!u)
+      return api.greedy(t->data_ptr(), xc.data_ptr(), tb, ip(pc), tokens.data_ptr(), pp, cp, st.s, (int)B, (int)N,
+                        (int)V, any_code(*t), stream);
+    return api.verify(t->data_ptr(), d ? d->data_ptr() : nullptr, xc.data_ptr(), tb, ip(pc), uc.data_ptr(),
+                      (int)uc.element_size(), tokens.data_ptr(), pp, cp, st.s, sd.s, (int)B, (int)N, (int)V,
+                      any_code(*t), replacement, stream);
+  });
+  if (rc) return PyLong_FromLong(rc);
+  PyObject *r0 = THPVariable_Wrap(tokens), *r1 = THPVariable_Wrap(path), *r2 = THPVariable_Wrap(counts);
+  return r0 && r1 && r2 ? Py_BuildValue("(NNN)", r0, r1, r2) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// keep(k_caches, v_caches, block_tables, starts, path, counts): lists of the layers' pools; True when done.
+PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !PyList_CheckExact(a[0]) || !PyList_CheckExact(a[1])) Py_RETURN_NONE;
+  const Py_ssize_t layers = PyList_GET_SIZE(a[0]);
+  if (layers < 1 || layers > 4096 || PyList_GET_SIZE(a[1]) != layers) Py_RETURN_NONE;
+  const Tensor* first[2] = {tensor(PyList_GET_ITEM(a[0], 0)), tensor(PyList_GET_ITEM(a[1], 0))};
+  const SeqPools P(first[0], first[1]);
+  if (!P.ok || dtype_code(*first[0]) < 0) Py_RETURN_NONE;
+  std::vector<void*> ptr[2];
+  for (int x = 0; x < 2; ++x) {
+    ptr[x].resize((size_t)layers);
+    for (Py_ssize_t l = 0; l < layers; ++l) {
+      const Tensor* t = tensor(PyList_GET_ITEM(a[x], l));
+      if (!t || !on_gpu(*t) || t->device() != first[0]->device() || t->scalar_type() != first[0]->scalar_type() ||
+          t->sizes() != first[x]->sizes() || t->strides() != first[x]->strides() ||
+          (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15))
+        Py_RETURN_NONE;
+      ptr[x][(size_t)l] = t->data_ptr();
+    }
+  }
+  const Tensor *bt = tensor(a[2]), *st = tensor(a[3]), *pa = tensor(a[4]), *cn = tensor(a[5]);
+  for (const Tensor* t : {bt, st, pa, cn})
+    if (!index_ok(t, *first[0])) Py_RETURN_NONE;
+  if (st->dim() != 1 || bt->dim() != 2 || pa->dim() != 2 || cn->dim() != 1) Py_RETURN_NONE;
+  const int64_t B = st->size(0);
+  if (bt->size(0) != B || pa->size(0) != B || cn->size(0) != B || !fits(B) || !fits(pa->size(1)) || !fits(bt->size(1)))
+    Py_RETURN_NONE;
+  const c10::OptionalDeviceGuard guard(first[0]->device());
+  const Tensor btc = index32(*bt), stc = index32(*st), pac = index32(*pa), cnc = index32(*cn);
+  void* stream = stream_of(*first[0]);
+  const int rc = launch([&] {
+    return api.keep(ptr[0].data(), ptr[1].data(), (int)layers, P.strides, P.strides + 3, ip(btc), ip(stc), ip(pac),
+                    pac.size(1), ip(cnc), (int)B, (int)pac.size(1), (int)first[0]->size(2), P.head_bytes,
+                    (int)first[0]->size(0), (int)first[0]->size(1), (int)btc.size(1), stream);
+  });
+  if (rc) return PyLong_FromLong(rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}): the library's entry points.
 PyObject* bind(PyObject*, PyObject* d) {
   void** out = reinterpret_cast<void**>(&api);
@@ -600,7 +784,8 @@ PyObject* names(PyObject*, PyObject*) {
 
 #define CIE_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CIE_FAST(flash), CIE_FAST(paged), CIE_FAST(section), CIE_FAST(append), CIE_FAST(append_seq),
-                         CIE_FAST(gather), CIE_FAST(int8),
+                         CIE_FAST(gather), CIE_FAST(int8), CIE_FAST(masks), CIE_FAST(tree), CIE_FAST(verify),
+                         CIE_FAST(keep),
                          {"bind", bind, METH_O, nullptr},
                          {"names", names, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

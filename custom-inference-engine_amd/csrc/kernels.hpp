@@ -221,6 +221,93 @@ int build_paged_plan(int32_t* P, const PagedGeom& g, const PlanLayout& L, const 
                      const int32_t* bt, int64_t bt_stride, int B, int Lq, int num_blocks, int block_size,
                      int max_blocks, int ctx_limit, int append);
 
+// Attention of a tree of N drafted tokens over the paged pool (tree_fwd.hip).
+constexpr int kTreeIds = 1024;       // block ids of a piece staged in LDS
+constexpr int kTreeMaxNodes = 1024;  // nodes of one tree
+struct TreeParams {
+  const uint16_t* q;
+  const uint16_t* kc;
+  const uint16_t* vc;
+  uint16_t* o;
+  const int32_t* bt;
+  const int32_t* lens;    // [B] history and nodes
+  const int32_t* mask;    // [B][N][W] bits of the nodes a node sees
+  const int32_t* depths;  // [B][N] (with rope)
+  int2* info;             // [B] first piece and pieces of a sequence (split launches)
+  float2* ml;             // [pieces][Hk][R] running maximum and sum of a piece's rows
+  float* part;            // [pieces][Hk][R][D] their unscaled outputs
+  int64_t qs0, qs1, qs2;  // batch, head, node
+  int64_t ks0, ks1, ks2;  // block, offset, head
+  int64_t vs0, vs1, vs2;
+  int64_t os0, os1, os2;
+  int64_t ms0, ms1, ds0;  // mask: batch, node; depths: batch
+  int B, Hk, N, W, group, R;  // R = group * N query rows per kv head
+  int num_blocks, max_blocks, block_size, ctx_limit;
+  FastDiv bsdiv, ndiv;    // by block_size, by N
+  int HG, NG, NRT, NCH, NST;  // kv heads per workgroup, head groups, row tiles, chunks per token row, ring stages
+  int extra, cmin;        // pieces beyond one per sequence; fewest tiles of a piece of a split sequence
+  int xcd_shift;
+  float scale_log2;       // as in PagedParams
+  uint32_t q_sign;
+  RopeTables rope;        // rotate q row of node i at position base + depths[i] as it is loaded
+  // Append (kn != nullptr): the nodes' rows b * N + i of kn / vn (strides per
+  // row and head) go into the pool first, K rotated like q.
+  const uint16_t* kn;
+  const uint16_t* vn;
+  int64_t kns0, kns1, vns0, vns1;
+  int D;
+  FastDiv updiv;          // by the chunk pairs of a token row, Hk * D / 16
+};
+
+// Launch geometry; a pure function of the arguments, so the workspace query
+// and the launch agree.
+struct TreeGeom {
+  int ok;
+  const char* err;
+  int R, QT, MW, HG, NG, NRT, NCH, NST;
+  int extra, cmin, wgs;
+  int split;  // a sequence may have several pieces: merge pass and workspace
+  size_t lds_bytes;
+  size_t info_bytes, ml_bytes, part_bytes;  // workspace parts
+};
+TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int block_size, DeviceShape dev);
+hipError_t launch_tree(const TreeParams& p, const TreeGeom& g, int dtype, int D, hipStream_t stream);
+
+// Draft trees (draft.hip).
+hipError_t launch_draft_masks(const int32_t* parents, int32_t* mask, int32_t* depths, uint32_t* status, int B, int N,
+                              hipStream_t stream);
+
+struct VerifyParams {
+  const void* target;  // (B, N, V) probabilities (greedy: logits), strides ts0, ts1, 1
+  const void* draft;   // (B, N, V) or nullptr
+  const void* draft_tokens;  // [B][N], token_bytes each (4 or 8)
+  const int32_t* parents;    // [B][N]
+  const void* uniforms;      // [B][N], uniform_bytes each (4 or 8)
+  void* tokens;              // [B][N] like draft_tokens
+  int32_t* path;             // [B][N]
+  int32_t* counts;           // [B]
+  int64_t ts0, ts1, ds0, ds1;
+  int token_bytes, uniform_bytes;
+  int B, N, V;
+};
+// mode: -1 greedy, 0 the draft's own picks, 1 drafts with replacement, 2 without; dtype as CIE_TABLE_*
+hipError_t launch_verify(const VerifyParams& p, int mode, int dtype, hipStream_t stream);
+
+constexpr int kKeepLayers = 64;  // layers of one launch (1 KiB of arguments)
+struct KeepParams {
+  const int32_t* bt;
+  const int32_t* starts;  // [B] position of node 0
+  const int32_t* path;    // [B][>= N], row stride ps0
+  const int32_t* counts;  // [B]
+  int64_t ps0;
+  int64_t block[2], token[2], head[2];  // byte strides of the K and V pools
+  int N, layers, max_blocks, num_blocks, block_size;
+  uint32_t cpr, cph;      // 16-byte chunks per token row, per head row
+  FastDiv cprdiv, cphdiv, bsdiv;
+  char* pools[2 * kKeepLayers];  // K and V of layer 0, of layer 1, ...
+};
+hipError_t launch_kv_keep(const KeepParams& p, int B, hipStream_t stream);
+
 // Paged KV append: new token rows (T, Hk, D) into the pool through block tables.
 struct AppendParams {
   const uint16_t* k_new;

@@ -55,6 +55,12 @@ EXPORTED_SYMBOLS = (
     "cie_paged_fwd_append",
     "cie_paged_fwd_append_rope",
     "cie_kv_append_rope",
+    "cie_draft_masks",
+    "cie_tree_workspace_bytes",
+    "cie_tree_attn",
+    "cie_verify_draft",
+    "cie_verify_greedy",
+    "cie_kv_keep",
     "cie_int8_matmul_workspace_bytes",
     "cie_int8_matmul",
 )
@@ -148,6 +154,21 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cie_kv_append_rope.argtypes = [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64p, _vp, _vp, _vp, _vp,
                                        _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _vp, _i64p, _vp]
     lib.cie_kv_append_rope.restype = _i
+    lib.cie_draft_masks.argtypes = [_vp, _vp, _vp, _vp, _i, _i, _vp]
+    lib.cie_draft_masks.restype = _i
+    lib.cie_tree_workspace_bytes.argtypes = [_i] * 8
+    lib.cie_tree_workspace_bytes.restype = ctypes.c_size_t
+    lib.cie_tree_attn.argtypes = [_vp] * 11 + [ctypes.c_size_t] + [_i64p] * 6 + [ctypes.c_int64] * 2 + [_i] * 9 + [
+        ctypes.c_float, _i, _vp, _vp, _i, _i, _vp]
+    lib.cie_tree_attn.restype = _i
+    lib.cie_verify_draft.argtypes = [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i64p, _i64p,
+                                     _i, _i, _i, _i, _i, _vp]
+    lib.cie_verify_draft.restype = _i
+    lib.cie_verify_greedy.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i64p, _i, _i, _i, _i, _vp]
+    lib.cie_verify_greedy.restype = _i
+    lib.cie_kv_keep.argtypes = [ctypes.POINTER(_vp), ctypes.POINTER(_vp), _i, _i64p, _i64p, _vp, _vp, _vp,
+                                ctypes.c_int64, _vp, _i, _i, _i, ctypes.c_int64, _i, _i, _i, _vp]
+    lib.cie_kv_keep.restype = _i
     lib.cie_int8_matmul_workspace_bytes.argtypes = [_i, _i, _i]
     lib.cie_int8_matmul_workspace_bytes.restype = ctypes.c_size_t
     lib.cie_int8_matmul.argtypes = [_vp, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,

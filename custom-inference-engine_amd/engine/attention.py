@@ -542,3 +542,126 @@ def paged_attention(
             rc = lib.cie_paged_fwd_rope(*args, *rope_args(rope, D, q.device), stream)
     _lib.check(rc)
     return out
+
+
+def tree_workspace_bytes(B: int, Hq: int, Hk: int, N: int, D: int, block_size: int, max_blocks_per_seq: int,
+                         max_context: int | None = None) -> int:
+    """Device workspace (bytes) a :func:`tree_attention` call of this shape
+    needs: the partial states of sequences split across workgroups."""
+    return int(_lib.load().cie_tree_workspace_bytes(B, Hq, Hk, N, D, int(max_context or 0), block_size,
+                                                    max_blocks_per_seq))
+
+
+def tree_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    tree_mask: torch.Tensor,
+    scale: float | None = None,
+    max_context: int | None = None,
+    *,
+    rope: tuple[torch.Tensor, torch.Tensor] | None = None,
+    depths: torch.Tensor | None = None,
+    new_kv: tuple[torch.Tensor, torch.Tensor] | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of a tree of N drafted tokens per sequence over its paged
+    history and their ancestors.
+
+    q: (B, Hq, N, D). Pools, block_tables, context_lens and max_context as in
+    :func:`paged_attention`; every context length counts the N nodes, which lie
+    at positions ``context_lens[b] - N + i``. tree_mask: int32
+    (B, N, ceil(N / 32)), or (N, ceil(N / 32)) for one tree of all sequences
+    (``engine.decode.draft_tree(parents).mask``): node i sees the history and
+    the nodes a whose bit a is set in its row. A row without a set bit is a
+    padding slot; its output is zero. Keys that a row does not see have no
+    influence on it, whatever the pool holds there. N is at most 1024. Returns
+    (B, Hq, N, D) in q's dtype; rows of a sequence with an invalid length or
+    block id are NaN.
+
+    ``rope``: (cos, sin) tables; q is then un-rotated, and node i is rotated at
+    position ``context_lens[b] - N + depths[b, i]`` as it is loaded (``depths``
+    int32 (B, N) or (N,), ``draft_tree(parents).depths``), bit-identical to
+    ``rope_apply`` at those positions first. ``new_kv``: (k_new, v_new), each
+    (B * N, Hk, D), row b * N + i = node i of sequence b, not yet in the pool:
+    they are written there first, K rotated as q when ``rope`` is given (rows of
+    padding slots are not written). ``out``: an existing (B, Hq, N, D) tensor to
+    write, as in :func:`flash_attention`.
+    """
+    cos, sin = rope if rope is not None else (None, None)
+    k_new, v_new = new_kv if new_kv is not None else (None, None)
+    done = _lib.host().tree(q, k_cache, v_cache, block_tables, context_lens, tree_mask, scale, max_context or 0, cos,
+                            sin, depths if rope is not None else None, out, k_new, v_new)
+    if done is not None:
+        return _lib.checked(done)
+    # everything else: refuse, copy or convert
+    given = [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
+             ("context_lens", context_lens), ("tree_mask", tree_mask)]
+    given += [(n, t) for n, t in (("depths", depths), ("k_new", k_new), ("v_new", v_new)) if t is not None]
+    for name, t in given:
+        if not t.is_cuda or t.device != q.device:
+            raise RuntimeError(f"tree_attention requires CUDA tensors on one device ({name})")
+    if q.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("tree_attention expects q (B,Hq,N,D) and pools (num_blocks,block_size,Hk,D)")
+    B, Hq, N, D = q.shape
+    _check_head_dim(D)
+    _check_dtype(q)
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"q and the KV pool must share a dtype, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    if tuple(k_cache.shape) != tuple(v_cache.shape) or k_cache.shape[-1] != D:
+        raise ValueError(f"pool shape mismatch: k {tuple(k_cache.shape)}, v {tuple(v_cache.shape)}, head_dim {D}")
+    num_blocks, block_size, Hk, _ = k_cache.shape
+    if Hk < 1 or Hq % Hk:
+        raise ValueError(f"num_heads {Hq} must be a multiple of num_kv_heads {Hk}")
+    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError(f"block_tables must be (B, max_blocks), got {tuple(block_tables.shape)}")
+    if context_lens.dim() != 1 or context_lens.shape[0] != B:
+        raise ValueError(f"context_lens must be (B,), got {tuple(context_lens.shape)}")
+    W = -(-N // 32)
+    if tree_mask.dtype != torch.int32 or tuple(tree_mask.shape) not in ((B, N, W), (N, W)):
+        raise ValueError(f"tree_mask must be int32 ({B}, {N}, {W}) or ({N}, {W}), got {tree_mask.dtype} "
+                         f"{tuple(tree_mask.shape)}")
+    if rope is not None and depths is None:
+        raise ValueError("tree_attention: rope needs the nodes' depths")
+    if rope is not None and (depths.dtype != torch.int32 or tuple(depths.shape) not in ((B, N), (N,))):
+        raise ValueError(f"depths must be int32 ({B}, {N}) or ({N},), got {depths.dtype} {tuple(depths.shape)}")
+    if new_kv is not None:
+        for name, t in (("k_new", k_new), ("v_new", v_new)):
+            if tuple(t.shape) != (B * N, Hk, D) or t.dtype != q.dtype:
+                raise ValueError(f"{name} must be ({B * N}, {Hk}, {D}) in {q.dtype}, got {tuple(t.shape)} {t.dtype}")
+        if _kernel_layout(k_cache) is not k_cache or _kernel_layout(v_cache) is not v_cache:
+            # the append writes the pools in place: a copy would drop the nodes
+            raise ValueError("tree_attention(new_kv=...) needs pools with a unit last stride, 16-byte aligned rows "
+                             "and outer strides in multiples of 8 elements")
+        k_new, v_new = _kernel_layout(k_new), _kernel_layout(v_new)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    lib = _lib.load()
+    bt = block_tables.to(torch.int32).contiguous()
+    lens = context_lens.to(torch.int32).contiguous()
+    mask = tree_mask if tree_mask.stride(-1) == 1 and tree_mask.stride(-2) == W else tree_mask.contiguous()
+    if depths is not None and depths.stride(-1) != 1:
+        depths = depths.contiguous()
+    q, k_cache, v_cache = _kernel_layout(q), _kernel_layout(k_cache), _kernel_layout(v_cache)
+    out = _output(out, (B, Hq, N, D), q)
+    mc = int(max_context or 0)
+    rp = rope_args(rope, D, q.device) if rope is not None else (None, None, 0, 0)
+    none3 = (ctypes.c_int64 * 3)(0, 0, 1)
+    with torch.cuda.device(q.device):
+        nbytes = int(lib.cie_tree_workspace_bytes(B, Hq, Hk, N, D, mc, block_size, bt.shape[1]))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        rc = lib.cie_tree_attn(
+            q.data_ptr(), k_new.data_ptr() if new_kv is not None else None,
+            v_new.data_ptr() if new_kv is not None else None, k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(),
+            lens.data_ptr(), mask.data_ptr(), depths.data_ptr() if rope is not None else None, out.data_ptr(),
+            ws.data_ptr() if ws is not None else None, nbytes, _lib.strides(q),
+            _lib.strides3(k_new) if new_kv is not None else none3, _lib.strides3(v_new) if new_kv is not None else none3,
+            _lib.strides(k_cache), _lib.strides(v_cache), _lib.strides(out),
+            mask.stride(0) if mask.dim() == 3 else 0,
+            depths.stride(0) if rope is not None and depths.dim() == 2 else 0,
+            B, Hq, Hk, N, D, num_blocks, block_size, bt.shape[1], mc, float(scale), _lib.DTYPE_CODES[q.dtype], *rp,
+            _lib.stream_handle(q.device))
+    _lib.check(rc)
+    return out

@@ -27,6 +27,7 @@ keeps the reference's slice copies, since no kernel runs there.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass, field
 from typing import Sequence
 
@@ -212,6 +213,61 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v
                 out_p, out_st = k_out.data_ptr(), _lib.strides3(k_out)
             rc = lib.cie_kv_append_rope(*args, *rope_args(rope, D, k_cache.device), out_p, out_st,
                                         _lib.stream_handle(k_cache.device))
+    _lib.check(rc)
+
+
+def kv_keep(k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor], block_tables: torch.Tensor,
+            starts: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> None:
+    """Move the K and V of accepted draft paths behind the histories, in every
+    layer's pools at once: the row at position ``starts[b] + path[b, j]`` goes
+    to ``starts[b] + j`` for j < ``counts[b]``.
+
+    k_caches / v_caches: the layers' pools, all of one shape, 16-bit type and
+    layout. block_tables (B, max_blocks), starts (B,), counts (B,): int32 or
+    int64 on the device; path (B, N), ``Verified.path``: rising, entry j at
+    least j. An entry outside [j, N) and a position whose block is out of range
+    move nothing."""
+    from engine import _lib
+
+    done = _lib.host().keep(k_caches, v_caches, block_tables, starts, path, counts)
+    if done is not None:
+        _lib.checked(done)
+        return
+    k_caches, v_caches = list(k_caches), list(v_caches)
+    if len(k_caches) != len(v_caches):
+        raise ValueError(f"kv_keep: {len(k_caches)} K pools and {len(v_caches)} V pools")
+    if not k_caches:
+        return
+    first = k_caches[0]
+    for t in [*k_caches, *v_caches, block_tables, starts, path, counts]:
+        if not t.is_cuda or t.device != first.device:
+            raise RuntimeError("kv_keep requires CUDA tensors on one device")
+    for pools in (k_caches, v_caches):
+        for t in pools:
+            if t.dim() != 4 or t.shape != first.shape or t.dtype != first.dtype or t.stride() != pools[0].stride():
+                raise ValueError("kv_keep expects pools (num_blocks, block_size, Hk, D) of one shape, dtype and layout")
+    if first.dtype not in _lib.DTYPE_CODES:
+        raise ValueError(f"attention kernels expect FP16 or BF16 Q/K/V, got {first.dtype}")
+    num_blocks, block_size, Hk, D = first.shape
+    if starts.dim() != 1 or path.dim() != 2 or path.shape[0] != starts.shape[0] or counts.shape != starts.shape \
+            or block_tables.dim() != 2 or block_tables.shape[0] != starts.shape[0]:
+        raise ValueError("kv_keep: block_tables must be (B, max_blocks), starts and counts (B,), path (B, N)")
+    for name, t in (("block_tables", block_tables), ("starts", starts), ("path", path), ("counts", counts)):
+        if t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"kv_keep: {name} must be int32 or int64, got {t.dtype}")
+    for t in (k_caches[0], v_caches[0]):
+        if t.stride(-1) != 1 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in range(3)):
+            raise ValueError("kv_keep needs pools with a unit last stride, 16-byte aligned rows and outer strides in "
+                             "multiples of 8 elements")
+    bt, st, pa, cn = (t.to(torch.int32).contiguous() for t in (block_tables, starts, path, counts))
+    n = len(k_caches)
+    ptrs = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in pools]) for pools in (k_caches, v_caches)]
+    byte_strides = [(ctypes.c_int64 * 3)(*[0 if t.shape[i] == 1 else 2 * t.stride(i) for i in range(3)])
+                    for t in (k_caches[0], v_caches[0])]
+    with torch.cuda.device(first.device):
+        rc = _lib.load().cie_kv_keep(*ptrs, n, *byte_strides, bt.data_ptr(), st.data_ptr(), pa.data_ptr(),
+                                     pa.shape[1], cn.data_ptr(), st.shape[0], pa.shape[1], Hk, 2 * D, num_blocks,
+                                     block_size, bt.shape[1], _lib.stream_handle(first.device))
     _lib.check(rc)
 
 
@@ -485,6 +541,21 @@ class PagedKVCache:
             self._free_block(bid)
         del table.blocks[keep:]
         table.length = new_length
+
+    def keep_step(self, step: "StepBatch", path: torch.Tensor, counts: torch.Tensor) -> None:
+        """The accepted paths of a step of draft trees (``Verified.path`` and
+        ``.counts`` on the device): :func:`kv_keep` over every layer. No host
+        work; :meth:`rollback_step` follows when the counts are known."""
+        kv_keep(self.k, self.v, step.block_tables, step.starts, path, counts)
+
+    def rollback_step(self, step: "StepBatch", counts: Sequence[int]) -> None:
+        """Shorten every sequence of a step to the first ``counts[b]`` of its
+        new tokens (host counts) and free the blocks no longer needed."""
+        counts = [int(c) for c in counts]
+        if len(counts) != len(step.tables) or any(not 0 <= c <= n for c, n in zip(counts, step.new_counts)):
+            raise ValueError(f"rollback_step: counts {counts} of a step with {list(step.new_counts)} new tokens")
+        for t, s0, c in zip(step.tables, step.starts_host, counts):
+            self.rollback(t, s0 + c)
 
     def stats(self) -> None:
         total = self.cfg.num_blocks

@@ -25,6 +25,9 @@ new tokens per sequence, e.g. a prefill chunk next to decode tokens) as
 packed rows: one append for all, then one launch per group of sequences with
 equal counts, ``paged_attention`` or ``paged_prefill`` by the same bound.
 
+:func:`tree_section` is the section of a speculative step whose drafts form a
+tree (``engine.decode``).
+
 The Lq new tokens of a sequence of context length ctx sit at positions
 ctx - Lq .. ctx - 1 (the reference appends before it attends,
 block.py:57-65), and row i sees keys <= ctx - Lq + i.
@@ -39,7 +42,7 @@ import math
 import torch
 
 from engine import _lib
-from engine.attention import flash_attention, paged_attention, paged_max_rows, paged_prefill
+from engine.attention import flash_attention, paged_attention, paged_max_rows, paged_prefill, tree_attention
 from engine.cache import PagedKVCache, StepBatch
 
 
@@ -139,6 +142,30 @@ def attention_section_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     cache.append_step(layer_idx, step, k, v, rope=rope)
     _paged_rows(q, layer_idx, cache, step, rope, out)
     return out.view(T, Hq * D)
+
+
+def tree_section(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layer_idx: int, cache: PagedKVCache,
+                 step: StepBatch, tree, rope: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """The attention section of a step of draft trees: q (B, Hq, N, D), k / v
+    (B, Hk, N, D) hold the N nodes of every sequence, un-rotated when ``rope``
+    is given; ``step`` is ``cache.prepare_step(tables, N)`` and ``tree``
+    ``engine.decode.draft_tree(parents)``, both made once per engine step. The
+    nodes' K and V are appended (K rotated at the node's position, history
+    length + depth) and every node attends over the history and its ancestors
+    (:func:`engine.attention.tree_attention`). Returns (B, N, Hq * D)."""
+    B, Hq, N, D = q.shape
+    if step.context_lens.shape[0] != B or k.shape[0] != B or v.shape[0] != B or step.num_new != N or not step.aligned:
+        raise ValueError(f"tree step of {step.context_lens.shape[0]} sequences x {step.num_new} nodes at the end of "
+                         f"every sequence expected for q of shape {tuple(q.shape)}")
+    Hk = k.shape[1]
+    cache._validate(k)
+    cache._validate(v)
+    out_rows = torch.empty((B, N, Hq, D), dtype=q.dtype, device=q.device)
+    tree_attention(q, cache.k[layer_idx], cache.v[layer_idx], step.block_tables, step.context_lens, tree.mask,
+                   max_context=step.max_context, rope=rope, depths=tree.depths,
+                   new_kv=(k.transpose(1, 2).reshape(B * N, Hk, D), v.transpose(1, 2).reshape(B * N, Hk, D)),
+                   out=out_rows.transpose(1, 2))
+    return out_rows.view(B, N, Hq * D)
 
 
 def _paged_rows(q_rows: torch.Tensor, layer_idx: int, cache: PagedKVCache, step: StepBatch,

@@ -491,6 +491,106 @@ int cie_int8_matmul(const void* x, const int8_t* w_int8, const void* scales, con
                     int M, int N, int K, int dtype, int scale_dtype,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Speculative decoding with draft trees (the reference drafts a single chain,
+ * engine/decode/speculative.py:47-133). A tree has N <= 1024 nodes given by
+ * parents, int32 [B, N]: node 0 is the last token the sequence has (parent
+ * -1), every other node comes after its parent; a parent below -1 marks a
+ * padding slot. Node i's K and V lie at position base + i behind a history of
+ * base tokens.
+ *
+ * cie_draft_masks: mask, int32 [B, N, (N + 31) / 32], bit a of row i set iff
+ * node a is node i or one of its ancestors; depths, int32 [B, N], the number
+ * of ancestors. Padding slots get an empty row and depth -1; so do, with depth
+ * -2 and 1 ORed into *status (optional device uint32), nodes whose chain to
+ * the root meets a padding slot or a parent that does not come before its child.
+ */
+int cie_draft_masks(const int32_t* parents, int32_t* mask, int32_t* depths, uint32_t* status, int B, int N,
+                    void* stream);
+
+/*
+ * Attention of the N nodes of every sequence over its paged history and their
+ * ancestors. q, o: (B, Hq, N, D); pools, block_tables and context_lens as in
+ * cie_paged_fwd, with every context length counting the N nodes (base =
+ * context_lens[b] - N). Node i sees the base tokens of the history and the
+ * nodes whose bit is set in row i of tree_mask (as cie_draft_masks lays it
+ * out; mask_batch_stride words between sequences, 0 for one tree for all). A
+ * row without a set bit is a padding slot: it sees nothing, its output is
+ * zero. What the pool holds at a position that a row does not see has no
+ * influence on the row, NaN and infinities included. A context length outside
+ * [N, limit] or a block id outside [0, num_blocks) is never dereferenced: the
+ * sequence's rows are NaN.
+ * rope_cos, rope_sin (NULL: none): q is un-rotated, node i is rotated at
+ * position base + depths[b][i] (depths_batch_stride ints between sequences).
+ * k_new, v_new (NULL: the nodes are in the pool): (B * N, Hk, D), row b * N +
+ * i = node i of sequence b, strides {row, head}; they are written into the
+ * pool first, K rotated like q. Rows of padding slots, of invalid sequences
+ * and of positions outside the rotary tables are not written (the last give
+ * NaN output rows).
+ * workspace: cie_tree_workspace_bytes bytes, 16-byte aligned, any contents,
+ * not shared by concurrent calls (0 bytes, NULL allowed, when no sequence can
+ * be split).
+ */
+size_t cie_tree_workspace_bytes(int B, int Hq, int Hk, int N, int D, int max_context, int block_size,
+                                int max_blocks_per_seq);
+int cie_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                  const int32_t* block_tables, const int32_t* context_lens, const int32_t* tree_mask,
+                  const int32_t* depths, void* o, void* workspace, size_t workspace_bytes,
+                  const int64_t* q_stride, const int64_t* kn_stride, const int64_t* vn_stride,
+                  const int64_t* kc_stride, const int64_t* vc_stride, const int64_t* o_stride,
+                  int64_t mask_batch_stride, int64_t depths_batch_stride, int B, int Hq, int Hk, int N, int D,
+                  int num_blocks, int block_size, int max_blocks_per_seq, int max_context, float scale, int dtype,
+                  const void* rope_cos, const void* rope_sin, int rope_rows, int rope_dtype, void* stream);
+
+/*
+ * Verification of a tree's drafted tokens. From node 0 on, the children of the
+ * current node are tried in index order; child i, token x, is accepted iff
+ * uniforms[i] * q(x) < p(x), p the target's probabilities at the current node
+ * and q the draft's. After a rejection p becomes max(p - q, 0) over its sum
+ * and, without replacement, q becomes q without x over its sum (each only if
+ * that sum is above 2^-40); draft_probs NULL: the drafts are the draft's own
+ * picks, q(x) = 1, and p loses x. When no child is accepted, the last token is
+ * the first y with p(0) + .. + p(y) > uniforms[0] * sum(p). All of it in 64 bits.
+ *   target_probs, draft_probs: (B, N, V) of type dtype (CIE_TABLE_*), strides
+ *       {sequence, node} in elements, unit vocabulary stride, any alignment;
+ *       row i = the distribution after node i (of its children)
+ *   draft_tokens: int32 or int64 [B, N] (token_bytes 4 or 8); a token outside
+ *       [0, V) is never accepted and changes nothing
+ *   uniforms: fp32 or fp64 [B, N] (uniform_bytes) in [0, 1)
+ *   path: int32 [B, N], node 0 and the accepted nodes, then -1
+ *   tokens: like draft_tokens, the accepted nodes' tokens and the last one,
+ *       then -1 (-1 as the last one where p has no positive entry)
+ *   counts: int32 [B], the entries of path and tokens; 0 for a sequence whose
+ *       node 0 is a padding slot
+ * Only the rows of the visited nodes are read. cie_verify_greedy: a child is
+ * accepted iff its token is the largest of target_logits at its parent (the
+ * lowest index of equal ones, a NaN the largest), which is also the last token.
+ * Reference: engine/decode/speculative.py:88-133 (greedy, one chain).
+ */
+int cie_verify_draft(const void* target_probs, const void* draft_probs, const void* draft_tokens, int token_bytes,
+                     const int32_t* parents, const void* uniforms, int uniform_bytes, void* tokens, int32_t* path,
+                     int32_t* counts, const int64_t* target_stride, const int64_t* draft_stride, int B, int N, int V,
+                     int dtype, int replacement, void* stream);
+int cie_verify_greedy(const void* target_logits, const void* draft_tokens, int token_bytes, const int32_t* parents,
+                      void* tokens, int32_t* path, int32_t* counts, const int64_t* target_stride, int B, int N, int V,
+                      int dtype, void* stream);
+
+/*
+ * Moves the K and V of the accepted path behind the history, in every layer:
+ * row starts[b] + path[b][j] of sequence b goes to row starts[b] + j, j <
+ * counts[b] (at most N). path[b][j] must be at least j and rise with j; an
+ * entry outside [j, N), a position outside the block table or a block id
+ * outside [0, num_blocks) moves nothing. k_caches, v_caches: `layers` device
+ * pointers in HOST memory, read during the call. Strides in bytes {block,
+ * token, head}, the same for every layer's K and every layer's V, multiples of
+ * 16; a head row is head_bytes bytes. path_stride: ints between sequences.
+ * Reference: engine/cache/kv_cache.py:187-194 rolls back a rejected chain.
+ */
+int cie_kv_keep(void* const* k_caches, void* const* v_caches, int layers, const int64_t* k_stride,
+                const int64_t* v_stride, const int32_t* block_tables, const int32_t* starts, const int32_t* path,
+                int64_t path_stride, const int32_t* counts, int B, int N, int heads, int64_t head_bytes,
+                int num_blocks, int block_size, int max_blocks_per_seq, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,10 @@ Contents
 ``int8_ref``       fp32 torch restatement of the reference's INT8 weight
                    path (``kernels/ref/int8_matmul_ref.py``,
                    ``kernels/int8_matmul.py``, ``engine/quant/calibrate.py``).
+``draft_ref``      draft trees in 64 bits: visibility, attention, the
+                   verification walk, the move of the accepted path (the
+                   reference drafts one chain and verifies it greedily,
+                   ``engine/decode/speculative.py:47-133``).
 ``brute``          fp64 numpy brute force written independently of the
                    above (explicit per-row max-subtracted exponentials).
 
@@ -41,6 +45,13 @@ from oracle.attention_ref import (  # noqa: F401
     paged_attention_ref,
 )
 from oracle.brute import attention_brute_f64, paged_attention_brute_f64  # noqa: F401
+from oracle.draft_ref import (  # noqa: F401
+    keep_ref,
+    mask_words,
+    tree_attention_f64,
+    tree_ref,
+    verify_ref,
+)
 from oracle.rope_ref import build_rope_cache_ref, rope_ref  # noqa: F401
 from oracle.int8_ref import (  # noqa: F401
     calibrate_weight_ref,
