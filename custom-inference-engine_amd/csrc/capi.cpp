@@ -1058,13 +1058,22 @@ int cie_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_c
   p.os0 = o_stride[0]; p.os1 = o_stride[1]; p.os2 = o_stride[2];
   p.W = (N + 31) / 32;
   p.ms0 = mask_batch_stride; p.ms1 = p.W; p.ds0 = depths_batch_stride;
-  p.B = B; p.Hk = Hk; p.N = N; p.group = Hq / Hk; p.R = g.R; p.D = D;
+  p.B = B; p.Hk = Hk; p.N = N; p.group = Hq / Hk; p.R = g.R; p.G32 = g.G32; p.D = D;
   p.num_blocks = num_blocks; p.max_blocks = max_blocks_per_seq; p.block_size = block_size; p.ctx_limit = ctx_limit;
   p.bsdiv = cie::make_fastdiv((uint32_t)block_size);
   p.ndiv = cie::make_fastdiv((uint32_t)N);
   p.updiv = cie::make_fastdiv((uint32_t)(Hk * D / 16));
   p.HG = g.HG; p.NG = g.NG; p.NRT = g.NRT; p.NCH = g.NCH; p.NST = g.NST;
   p.extra = g.extra; p.cmin = g.cmin;
+  {
+    const int64_t extent = 2 * ((int64_t)(num_blocks > 0 ? num_blocks - 1 : 0) * kc_stride[0] +
+                                (int64_t)(block_size - 1) * kc_stride[1] + (int64_t)(Hk - 1) * kc_stride[2] + D);
+    const int64_t lim24 = (int64_t)1 << 24;
+    p.narrow = extent < ((int64_t)1 << 31) && num_blocks < lim24 && 2 * kc_stride[0] < lim24 &&
+               kc_stride[0] == vc_stride[0] && kc_stride[1] == vc_stride[1] && kc_stride[2] == vc_stride[2] &&
+               (block_size % cie::kPagedTile == 0 || cie::kPagedTile % block_size == 0);
+    p.ks0_24 = (uint32_t)(2 * kc_stride[0]);
+  }
   p.xcd_shift = cie::device_shape().xcd_shift;
   set_scale(scale, &p.scale_log2, &p.q_sign);
   if (rope_cos) p.rope = cie::RopeTables{rope_cos, rope_sin, rope_rows, rope_dtype};

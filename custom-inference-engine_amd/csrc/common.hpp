@@ -260,6 +260,15 @@ __device__ __forceinline__ u32x2 lds_read_tr16(const void* lds_ptr) {
   return __builtin_bit_cast(u32x2, r);
 }
 
+// The same reads (and a plain 16-byte one) from an LDS byte address.
+__device__ __forceinline__ u32x2 lds_read_tr16_at(uint32_t addr) {
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)addr);
+  return __builtin_bit_cast(u32x2, r);
+}
+__device__ __forceinline__ u32x4 lds_read16_at(uint32_t addr) {
+  return *(__attribute__((address_space(3))) const u32x4*)(size_t)addr;
+}
+
 // Explicit waits are inline assembly so no compiler pass can relax them.
 template <int N>
 __device__ __forceinline__ void vm_wait() {

@@ -224,6 +224,14 @@ int build_paged_plan(int32_t* P, const PagedGeom& g, const PlanLayout& L, const 
 // Attention of a tree of N drafted tokens over the paged pool (tree_fwd.hip).
 constexpr int kTreeIds = 1024;       // block ids of a piece staged in LDS
 constexpr int kTreeMaxNodes = 1024;  // nodes of one tree
+constexpr int kTreeOddWords = kTreeMaxNodes / 32 + 2;  // tiles that reach past the history
+// Most threads of a workgroup with QT waves to a kv head: heads of at most 256
+// elements in all, eight waves (two to a SIMD; at D = 256 a wave needs a SIMD's
+// registers for itself).
+__host__ __device__ constexpr int tree_threads(int D, int QT) {
+  const int heads = 256 / D < 8 / QT ? 256 / D : 8 / QT;
+  return D == 256 ? 256 : 64 * QT * (heads < 1 ? 1 : heads);
+}
 struct TreeParams {
   const uint16_t* q;
   const uint16_t* kc;
@@ -234,17 +242,19 @@ struct TreeParams {
   const int32_t* mask;    // [B][N][W] bits of the nodes a node sees
   const int32_t* depths;  // [B][N] (with rope)
   int2* info;             // [B] first piece and pieces of a sequence (split launches)
-  float2* ml;             // [pieces][Hk][R] running maximum and sum of a piece's rows
-  float* part;            // [pieces][Hk][R][D] their unscaled outputs
+  float2* ml;             // [pieces][Hk][G32][32] running maximum and sum of a piece's rows
+  float* part;            // [pieces][Hk][G32][D / 8][64 lanes][4] their unscaled outputs
   int64_t qs0, qs1, qs2;  // batch, head, node
   int64_t ks0, ks1, ks2;  // block, offset, head
   int64_t vs0, vs1, vs2;
   int64_t os0, os1, os2;
   int64_t ms0, ms1, ds0;  // mask: batch, node; depths: batch
-  int B, Hk, N, W, group, R;  // R = group * N query rows per kv head
+  int B, Hk, N, W, group, R, G32;  // R = group * N query rows per kv head, in G32 groups of 32
   int num_blocks, max_blocks, block_size, ctx_limit;
   FastDiv bsdiv, ndiv;    // by block_size, by N
   int HG, NG, NRT, NCH, NST;  // kv heads per workgroup, head groups, row tiles, chunks per token row, ring stages
+  int narrow;             // K and V pools alike, 32-bit byte offsets, blocks and tiles that divide one another
+  uint32_t ks0_24;        // then: bytes of a block
   int extra, cmin;        // pieces beyond one per sequence; fewest tiles of a piece of a split sequence
   int xcd_shift;
   float scale_log2;       // as in PagedParams
@@ -264,7 +274,7 @@ struct TreeParams {
 struct TreeGeom {
   int ok;
   const char* err;
-  int R, QT, MW, HG, NG, NRT, NCH, NST;
+  int R, G32, QT, HG, NG, NRT, NCH, NST;
   int extra, cmin, wgs;
   int split;  // a sequence may have several pieces: merge pass and workspace
   size_t lds_bytes;

@@ -9,10 +9,10 @@
 //
 // Rows. The R = (Hq / Hk) * N query rows of a kv head are packed, r = g * N + i
 // (query head kvh * group + g), so that every K / V byte a workgroup stages
-// serves all of them. A wave holds MW groups of 32 rows (one row per lane pair,
-// see common.hpp), QT waves side by side cover a row tile of 32 QT MW rows of
-// one kv head, and a workgroup takes HG kv heads: HG * QT waves. Rows beyond
-// one tile go to workgroups of their own.
+// serves all of them. A wave holds 32 rows (one row per lane pair, see
+// common.hpp), QT waves side by side cover a row tile of 32 QT rows of one kv
+// head, and a workgroup takes HG kv heads: HG * QT waves. Rows beyond one tile
+// go to workgroups of their own.
 //
 // Keys. A piece, one workgroup's work, is a run of 32-token tiles of ONE
 // sequence. Every workgroup finds its own from the context lengths: with C the
@@ -23,7 +23,7 @@
 // combines in a fixed order.
 //
 // Per tile: K and V go global -> LDS by 16-byte direct copies into a ring of NST
-// stages (one barrier per tile: the stage refilled after it was read before it),
+// stages,
 //   S^T = K Q^T, online softmax in registers, O^T += V^T P^T
 // as in paged_fwd.hip. Only tiles that reach past the history look at the tree
 // mask: a lane cuts the 32 bits of the tile out of its row's words.
@@ -33,8 +33,10 @@
 //
 // A masked key must not reach a row even if its V holds infinities or NaN (the
 // slots of padding nodes are never written): in a tile past the history such
-// values are taken out of the product and added for the rows that see their key.
+// values are taken out in LDS before the product and added at the end for the rows
+// that see their key.
 #include <climits>
+#include <type_traits>
 
 #include "kernels.hpp"
 #include "rope.hpp"
@@ -124,13 +126,16 @@ __device__ __forceinline__ void tree_fill(uint16_t* row, int hl, uint32_t bits2)
     *reinterpret_cast<u32x4*>(row + d) = u32x4{bits2, bits2, bits2, bits2};
 }
 
-template <int DTYPE, int D, int QT, int MW>
-__global__ __launch_bounds__(256) void tree_fwd_kernel(const TreeParams p) {
+template <int DTYPE, int D, int QT>
+__global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const TreeParams p) {
   warm_kernargs<sizeof(TreeParams)>();
   using C = TreeCfg<D, QT>;
   using E = Elt<DTYPE>;
-  extern __shared__ __attribute__((aligned(16))) uint16_t ring[];
-  __shared__ int32_t sbt[kTreeIds];
+  // the ring first (its stages then lie at multiples of their power-of-two size,
+  // so that the swizzles below are an XOR of the address), the block ids behind it
+  extern __shared__ __attribute__((aligned(1024))) uint16_t ring[];
+  int32_t* const sbt = reinterpret_cast<int32_t*>(ring + p.NST * (2 * kPagedTile * 8) * p.NCH);
+  uint32_t* const odd = reinterpret_cast<uint32_t*>(sbt + kTreeIds);  // [HG][kTreeOddWords] keys whose V is not finite
 
   // (piece j, head group gh) = unit u, row tile rt; the row tiles of a unit are
   // 2^xcd_shift workgroup ids apart, so that they share an XCD's L2
@@ -181,25 +186,17 @@ __global__ __launch_bounds__(256) void tree_fwd_kernel(const TreeParams p) {
   if (b < 0) return;  // the launch has a workgroup for every piece there can be
   if (p.info && j == j0 && gh == 0 && rt == 0 && threadIdx.x == 0) p.info[b] = int2{j0, n};
 
-  // ---- query rows ------------------------------------------------------------
-  int node[MW], hq[MW];
-  bool rv[MW], live[MW];
-  const int32_t* words[MW];
-  uint16_t* orow[MW];
-#pragma unroll
-  for (int m = 0; m < MW; ++m) {
-    const int r = ((rt * QT + qt) * MW + m) * 32 + l32;
-    rv[m] = r < p.R;
-    const int g = rv[m] ? (int)fdiv((uint32_t)r, p.ndiv) : 0;
-    node[m] = rv[m] ? r - g * p.N : 0;
-    hq[m] = kvh * p.group + g;
-    words[m] = p.mask + (int64_t)b * p.ms0 + (int64_t)node[m] * p.ms1;
-    orow[m] = p.o + (int64_t)b * p.os0 + hq[m] * p.os1 + (int64_t)node[m] * p.os2;
-  }
+  // ---- query row -------------------------------------------------------------
+  const int r = (rt * QT + qt) * 32 + l32;
+  const bool rv = r < p.R;
+  const int g = rv ? (int)fdiv((uint32_t)r, p.ndiv) : 0;
+  const int node = rv ? r - g * p.N : 0;
+  const int hq = kvh * p.group + g;
+  const int32_t* const words = p.mask + (int64_t)b * p.ms0 + (int64_t)node * p.ms1;
+  auto out_row = [&] { return p.o + (int64_t)b * p.os0 + hq * p.os1 + (int64_t)node * p.os2; };
+  const bool live = tree_row_live(words, p.N);
   if (t == 0) {  // an invalid context length
-#pragma unroll
-    for (int m = 0; m < MW; ++m)
-      if (rv[m]) tree_fill<D>(orow[m], hl, tree_row_live(words[m], p.N) ? nan2 : 0u);
+    if (rv) tree_fill<D>(out_row(), hl, live ? nan2 : 0u);
     return;
   }
   const int per_piece = (int)(((uint32_t)t + (uint32_t)n - 1) / (uint32_t)n);
@@ -209,36 +206,27 @@ __global__ __launch_bounds__(256) void tree_fwd_kernel(const TreeParams p) {
   // ---- block ids of the piece ------------------------------------------------
   const int blk_lo = (int)fdiv((uint32_t)(kPagedTile * tlo), p.bsdiv);
   const int nids = (int)fdiv((uint32_t)(min(ctx, kPagedTile * thi) - 1), p.bsdiv) - blk_lo + 1;
-  bool bad = false;
   {
     const int32_t* src = p.bt + (int64_t)b * p.max_blocks + blk_lo;
     for (int x = threadIdx.x; x < nids; x += blockDim.x) {
       const int id = src[x];
-      const bool ok = (uint32_t)id < (uint32_t)p.num_blocks;
-      bad |= !ok;
-      sbt[x] = ok ? id : -1;
+      sbt[x] = (uint32_t)id < (uint32_t)p.num_blocks ? id : -1;
     }
   }
 
-  u32x4 qf[MW][C::KK];
+  u32x4 qf[C::KK];
+  const uint16_t* const qrow = p.q + (int64_t)b * p.qs0 + hq * p.qs1 + (int64_t)node * p.qs2;
 #pragma unroll
-  for (int m = 0; m < MW; ++m) {
-    const uint16_t* qrow = p.q + (int64_t)b * p.qs0 + hq[m] * p.qs1 + (int64_t)node[m] * p.qs2;
+  for (int kk = 0; kk < C::KK; ++kk) qf[kk] = load16(qrow + 16 * kk + 8 * hl, rv);
+  if (p.rope.cos)  // node i is rotated at position base + its depth
+    rope_q_lane<DTYPE, D>(qf, p.rope, base + max(p.depths[(int64_t)b * p.ds0 + node], 0), rv, hl);
 #pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) qf[m][kk] = load16(qrow + 16 * kk + 8 * hl, rv[m]);
-    live[m] = tree_row_live(words[m], p.N);
-  }
-  if (p.rope.cos) {
-    // node i is rotated at position base + its depth
-#pragma unroll
-    for (int m = 0; m < MW; ++m)
-      rope_q_lane<DTYPE, D>(qf[m], p.rope, base + max(p.depths[(int64_t)b * p.ds0 + node[m]], 0), rv[m], hl);
-  }
-#pragma unroll
-  for (int m = 0; m < MW; ++m)
-#pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) qf[m][kk] ^= u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
-  const bool poison = __syncthreads_or(bad);  // an id outside the pool: NaN rows, never a read
+  for (int kk = 0; kk < C::KK; ++kk) qf[kk] ^= u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
+  for (int x = threadIdx.x; x < p.HG * kTreeOddWords; x += blockDim.x) odd[x] = 0;
+  __syncthreads();
+  bool bad = false;
+  for (int x = lane; x < nids; x += 64) bad |= sbt[x] < 0;
+  const bool poison = __builtin_amdgcn_ballot_w64(bad) != 0;  // an id outside the pool: NaN rows, never a read
 
   // ---- copies ----------------------------------------------------------------
   const int NCH = p.NCH, NST = p.NST;
@@ -247,17 +235,23 @@ __global__ __launch_bounds__(256) void tree_fwd_kernel(const TreeParams p) {
   const int STAGE_EL = 2 * TILE_EL;
   const bool issuer = qt < C::QTI;
   const int c0 = (hh * C::QTI + qt) * C::CPW;  // this wave's first copy of a tensor's tile
-  int ltok[C::CPW];
-  int32_t goffk[C::CPW], goffv[C::CPW];
+  // chunk P = 64 (c0 + x) + lane of the tile: token P / NCH, stored chunk P % NCH of
+  // its row, which holds chunk (P % NCH) ^ row_swizzle(token); NCH divides 64
+  const int tok0 = (64 * c0 + lane) >> lg_nch, tok_step = 64 >> lg_nch, chunk0 = lane & (NCH - 1);
+  const uint16_t* const kbase = p.kc + (int64_t)gh * p.HG * p.ks2;
+  const uint16_t* const vbase = p.vc + (int64_t)gh * p.HG * p.vs2;
+  // Whole tiles of a pool that 32-bit byte offsets reach, K and V laid out alike,
+  // blocks a multiple or a divisor of the tile: per copy one block id and one
+  // multiply-add, everything else of the address is the lane's own (without this
+  // the addresses took more of a step than its softmax).
+  uint32_t lofs[C::CPW];
+  int lblk[C::CPW];
 #pragma unroll
   for (int x = 0; x < C::CPW; ++x) {
-    const int P = 64 * (c0 + x) + lane;
-    const int tk = P >> lg_nch;
-    const int c = (P & (NCH - 1)) ^ row_swizzle(NCH, tk & (kPagedTile - 1));
-    const int hd = c / C::S, dc = c % C::S;
-    ltok[x] = tk;
-    goffk[x] = (gh * p.HG + hd) * (int32_t)p.ks2 + 8 * dc;
-    goffv[x] = (gh * p.HG + hd) * (int32_t)p.vs2 + 8 * dc;
+    const int tk = tok0 + x * tok_step;
+    const int cx = chunk0 ^ row_swizzle(NCH, tk);
+    lblk[x] = (int)fdiv((uint32_t)tk, p.bsdiv);
+    lofs[x] = 2u * (uint32_t)((tk - lblk[x] * p.block_size) * (int)p.ks1 + (cx / C::S) * (int)p.ks2 + 8 * (cx % C::S));
   }
   const uint32_t ring_lds = lds_addr_of(ring);
   int i_stage = 0;
@@ -265,191 +259,234 @@ __global__ __launch_bounds__(256) void tree_fwd_kernel(const TreeParams p) {
     const int tbase = kPagedTile * (tlo + k);
     const uint32_t st = ring_lds + 2u * (uint32_t)(i_stage * STAGE_EL) + 1024u * (uint32_t)c0;
     i_stage = i_stage + 1 == NST ? 0 : i_stage + 1;
-    int bid[C::CPW], off[C::CPW];
+    if (p.narrow && tbase + kPagedTile <= ctx) {
+      const int blk = (int)fdiv((uint32_t)tbase, p.bsdiv);
+      const uint32_t in = 2u * (uint32_t)((tbase - blk * p.block_size) * (int)p.ks1);  // 0 unless blocks are larger
+      uint32_t off[C::CPW];
 #pragma unroll
-    for (int x = 0; x < C::CPW; ++x) {
-      const int tk = min(tbase + ltok[x], ctx - 1);
-      const int blk = (int)fdiv((uint32_t)tk, p.bsdiv);
-      off[x] = tk - blk * p.block_size;
-      bid[x] = max(sbt[blk - blk_lo], 0);
+      for (int x = 0; x < C::CPW; ++x)
+        off[x] = __umul24((uint32_t)max(sbt[blk - blk_lo + lblk[x]], 0), p.ks0_24) + lofs[x] + in;
+#pragma unroll
+      for (int x = 0; x < C::CPW; ++x) {
+        dma16_sv_nt(kbase, off[x], st + 1024u * x);
+        dma16_sv_nt(vbase, off[x], st + 2u * TILE_EL + 1024u * x);
+      }
+      return;
     }
-#pragma unroll
     for (int x = 0; x < C::CPW; ++x) {
-      dma16_at_nt(p.kc + (int64_t)bid[x] * p.ks0 + (int64_t)off[x] * p.ks1 + goffk[x], st + 1024u * x);
-      dma16_at_nt(p.vc + (int64_t)bid[x] * p.vs0 + (int64_t)off[x] * p.vs1 + goffv[x], st + 2u * TILE_EL + 1024u * x);
+      const int tk = min(tbase + tok0 + x * tok_step, ctx - 1);
+      const int blk = (int)fdiv((uint32_t)tk, p.bsdiv), off = tk - blk * p.block_size;
+      const int bid = max(sbt[blk - blk_lo], 0);
+      const int cx = chunk0 ^ row_swizzle(NCH, tok0 + x * tok_step);
+      const int hd = cx / C::S, dc = 8 * (cx % C::S);
+      dma16_at_nt(kbase + (int64_t)bid * p.ks0 + (int64_t)off * p.ks1 + hd * (int32_t)p.ks2 + dc, st + 1024u * x);
+      dma16_at_nt(vbase + (int64_t)bid * p.vs0 + (int64_t)off * p.vs1 + hd * (int32_t)p.vs2 + dc,
+                  st + 2u * TILE_EL + 1024u * x);
     }
   };
+  const int reach = NST - 1;  // step k copies tile k + reach
   if (issuer)
-    for (int k = 0; k < min(NST - 1, T); ++k) issue(k);
+    for (int k = 0; k < min(reach, T); ++k) issue(k);
 
   // ---- tile loop -------------------------------------------------------------
-  const int swk = row_swizzle(NCH, l32);
-  const int rq = lane & 15, gq = lane >> 4;
-  int swv[2][2];
+  // Byte addresses inside a tile. K row l32, chunk hh S + 2 kk + hl: the kk part is
+  // an XOR of the address. V^T fragment (dt, cc): lane (group gq, row rq of it) points
+  // at token 16 cc + 4 hl + rq / 4 (and 8 on), dims 32 dt + 16 (gq & 1) + 4 (rq % 4)
+  // (the dt part an XOR too); the transpose read hands each lane four keys of dim
+  // 32 dt + l32.
+  const uint32_t k_lane = 16u * (uint32_t)((l32 << lg_nch) + ((hh * C::S + hl) ^ row_swizzle(NCH, l32)));
+  uint32_t v_lane[2][2];
+  {
+    const int rq = lane & 15, gq = lane >> 4;
+    int d = 16 * (gq & 1) + 4 * (rq & 3);
+    if (D < 32) d = min(d, D - 4);  // rows >= D of O^T are discarded
 #pragma unroll
-  for (int cc = 0; cc < 2; ++cc) {
-    swv[cc][0] = row_swizzle(NCH, 16 * cc + 4 * hl + (rq >> 2));
-    swv[cc][1] = row_swizzle(NCH, 16 * cc + 4 * hl + (rq >> 2) + 8);
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int up = 0; up < 2; ++up) {
+        const int tk = 16 * cc + 4 * hl + (rq >> 2) + 8 * up;
+        v_lane[cc][up] = 2u * (uint32_t)TILE_EL +
+                         16u * (uint32_t)((tk << lg_nch) + ((hh * C::S + (d >> 3)) ^ row_swizzle(NCH, tk))) + 2u * (d & 7);
+      }
   }
-  f32x16 acc[MW][C::DT];
-  float mx[MW], l[MW];
+  f32x16 acc[C::DT];
 #pragma unroll
-  for (int m = 0; m < MW; ++m) {
-#pragma unroll
-    for (int dt = 0; dt < C::DT; ++dt) acc[m][dt] = f32x16{};
-    mx[m] = -INFINITY;
-    l[m] = 0.f;
-  }
+  for (int dt = 0; dt < C::DT; ++dt) acc[dt] = f32x16{};
+  float mx = -INFINITY, l = 0.f;
   const float c = p.scale_log2;
-  int c_stage = 0;
+  const int whole = min(max(base / kPagedTile - tlo, 0), T);  // tiles of history alone
+  f32x16 sc = f32x16{};        // scores of the tile, then its probabilities
+  u32x4 pb[2] = {};            // those in 16 bits
 
-  for (int k = 0; k < T; ++k) {
-    if (issuer) tree_wait<2 * C::CPW>(min(NST - 2, T - 1 - k));
-    __syncthreads();  // tile k is in LDS for every wave, and every wave is done with tile k - 1
-    if (issuer && k + NST - 1 < T) issue(k + NST - 1);
-    const uint16_t* kst = ring + c_stage * STAGE_EL;
-    const uint16_t* vst = kst + TILE_EL;
-    c_stage = c_stage + 1 == NST ? 0 : c_stage + 1;
-    const int t0 = kPagedTile * (tlo + k);
-
-    f32x16 sc[MW];
-#pragma unroll
-    for (int m = 0; m < MW; ++m) sc[m] = f32x16{};
-#pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) {
-      const int pos = (hh * C::S + 2 * kk + hl) ^ swk;
-      const u32x4 a = *reinterpret_cast<const u32x4*>(kst + ((l32 << lg_nch) + pos) * 8);
-#pragma unroll
-      for (int m = 0; m < MW; ++m) sc[m] = E::mfma(a, qf[m][kk], sc[m]);
+  // V of a tile past the history, before any wave reads it: values that are not
+  // finite become zeros in LDS and their keys are noted, this wave's share of the
+  // tile's tokens.
+  auto tidy = [&](int k, int st) __attribute__((always_inline)) {
+    uint16_t* const vst = ring + st * STAGE_EL + TILE_EL;
+    constexpr int TOK = kPagedTile / QT;
+    for (int x = lane; x < TOK * C::S; x += 64) {
+      const int tk = qt * TOK + x / C::S, cc = (hh * C::S + x % C::S) ^ row_swizzle(NCH, tk);
+      u32x4* const at = reinterpret_cast<u32x4*>(vst + ((tk << lg_nch) + cc) * 8);
+      const u32x4 v = *at;
+      if (!all_finite<DTYPE>(v)) {
+        *at = finite_or_zero<DTYPE>(v);
+        atomicOr(&odd[hh * kTreeOddWords + (k - whole)], 1u << tk);
+      }
     }
-    const bool tail = t0 + kPagedTile > base;
-    uint32_t vis[MW], odd_keys = 0;
-    bool odd = false;
-    if (tail) {
+  };
+  // Step k: the matrix part, scores of tile k and values of tile k - 1, then the
+  // softmax of tile k. Fragments are read from LDS ahead of their products: V of tile
+  // k - 1 between the products of the scores, K of tile k + 1 between the pieces of
+  // the softmax (read right before use, the LDS latency stood in front of every
+  // product; read all at once, the LDS bandwidth in front of the rest).
+  //
+  // One barrier a step, between the two parts: behind it every wave has read V of tile
+  // k - 1 (whose stage the softmax part refills) and every wave's copies of tile k + 1
+  // are done. (Eight waves in two halves, one in its matrix part while the other is in
+  // its softmax, kept apart by a barrier after each part: 88 -> 90 us for four trees of
+  // 64 nodes over 8192-16384 tokens, 42 -> 51 for 32 of 16 over 256-4096; the halves
+  // wait for one another more than they overlap.)
+  u32x4 vf[2 * C::DT], kf[C::KK];
+  auto load_key = [&](int st, int kk) __attribute__((always_inline)) {
+    kf[kk] = lds_read16_at((ring_lds + 2u * (uint32_t)(st * STAGE_EL) + k_lane) ^ (32u * kk));
+  };
+  auto load_value = [&](int st, int f) __attribute__((always_inline)) {
+    const uint32_t sp = ring_lds + 2u * (uint32_t)(st * STAGE_EL);
+    const u32x2 lo = lds_read_tr16_at((sp + v_lane[f & 1][0]) ^ (64u * (f >> 1)));
+    const u32x2 hi = lds_read_tr16_at((sp + v_lane[f & 1][1]) ^ (64u * (f >> 1)));
+    vf[f] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  if (issuer) tree_wait<2 * C::CPW>(min(reach - 1, T - 1));
+  __syncthreads();
 #pragma unroll
-      for (int m = 0; m < MW; ++m) {
-        vis[m] = tree_bits(words[m], t0 - base, p.N, p.W, live[m]);
-        const uint32_t mine = vis[m] >> (4 * hl);
+  for (int kk = 0; kk < C::KK; ++kk) load_key(0, kk);
+  if (whole == 0) tidy(0, 0);
+  int st_cur = 0, st_prev = 0;  // stages of tiles k and k - 1
+  for (int k = 0; k <= T; ++k) {
+    sc = f32x16{};
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          sc[m][e] = (mine >> (8 * (e >> 2) + (e & 3))) & 1u ? sc[m][e] : -INFINITY;
-      }
-      // keys of this head whose V has a value that is not finite
-      odd_keys = 0;
-      for (int x = lane; x < kPagedTile * C::S; x += 64) {
-        const int tk = x / C::S, cc = (hh * C::S + x % C::S) ^ row_swizzle(NCH, tk);
-        const u32x4 v = *reinterpret_cast<const u32x4*>(vst + ((tk << lg_nch) + cc) * 8);
-        if (!all_finite<DTYPE>(v)) odd_keys |= 1u << tk;
-      }
-      odd = __builtin_amdgcn_ballot_w64(odd_keys != 0) != 0;
-      if (odd)
-        for (int x = 1; x < 64; x *= 2) odd_keys |= (uint32_t)__shfl_xor((int)odd_keys, x);
+    for (int kk = 0; kk < C::KK; ++kk) {  // (k = T: a product of no use)
+      sc = E::mfma(kf[kk], qf[kk], sc);
+      if (kk < 2 * C::DT) load_value(st_prev, kk);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    u32x4 pb[MW][2];
-#pragma unroll
-    for (int m = 0; m < MW; ++m) {
-      const float mxs = xhalf_max(max16(sc[m])) * c;
-      const bool grow = mxs > mx[m] + kLazyRescaleTree;
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-        const float m_new = grow ? mxs : mx[m];
-        const float alpha = grow ? exp2_fast(mx[m] - m_new) : 1.f;
-        l[m] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < C::DT; ++dt) acc[m][dt] *= alpha;
-        mx[m] = m_new;
-      }
-      const float neg_m = mx[m] == -INFINITY ? 0.f : -mx[m];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[m][e] = exp2_fast(fmaf(sc[m][e], c, neg_m));
-      l[m] += sum16(sc[m]);
+    if (D < 32) load_value(st_prev, 1);
+    if (k > 0) {
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) pb[m][cc][x] = E::pack2(sc[m][8 * cc + 2 * x], sc[m][8 * cc + 2 * x + 1]);
+        for (int dt = 0; dt < C::DT; ++dt) acc[dt] = E::mfma(vf[2 * dt + cc], pb[cc], acc[dt]);
+      if (k == T) break;
     }
+    const int st_next = st_cur + 1 == NST ? 0 : st_cur + 1;
+    if (issuer && k + 1 < T) tree_wait<2 * C::CPW>(min(reach - 2, T - 2 - k));
+    __syncthreads();
+    if (issuer && k + reach < T) issue(k + reach);
+    if (k + 1 >= whole && k + 1 < T) tidy(k + 1, st_next);
+    if (k >= whole) {  // the tile reaches past the history: the row's mask decides
+      const uint32_t vis = tree_bits(words, kPagedTile * (tlo + k) - base, p.N, p.W, live) >> (4 * hl);
 #pragma unroll
-    for (int dt = 0; dt < C::DT; ++dt) {
-      int d = 32 * dt + 16 * (gq & 1) + 4 * (rq & 3);
-      if (D < 32) d = min(d, D - 4);  // rows >= D of O^T are discarded
-      const int chunk = hh * C::S + (d >> 3), within = d & 7;
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
-        const int tl = 16 * cc + 4 * hl + (rq >> 2), th = tl + 8;
-        const u32x2 lo = lds_read_tr16(vst + ((tl << lg_nch) + (chunk ^ swv[cc][0])) * 8 + within);
-        const u32x2 hi = lds_read_tr16(vst + ((th << lg_nch) + (chunk ^ swv[cc][1])) * 8 + within);
-        u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
-        if (odd) a = finite_or_zero<DTYPE>(a);
-#pragma unroll
-        for (int m = 0; m < MW; ++m) acc[m][dt] = E::mfma(a, pb[m][cc], acc[m][dt]);
-      }
+      for (int e = 0; e < 16; ++e) sc[e] = (vis >> (8 * (e >> 2) + (e & 3))) & 1u ? sc[e] : -INFINITY;
     }
-    // the values left out, for the rows that see their key
-    for (uint32_t keys = odd ? __builtin_amdgcn_readfirstlane(odd_keys) : 0u; keys; keys &= keys - 1) {
-      const int tk = __builtin_ctz(keys), es = 4 * (tk >> 3) + (tk & 3);
-      const uint16_t* vrow = vst + (tk << lg_nch) * 8;
-      const int sw = row_swizzle(NCH, tk);
+    const float mxs = xhalf_max(max16(sc)) * c;
+    const bool grow = mxs > mx + kLazyRescaleTree;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float m_new = grow ? mxs : mx;
+      const float alpha = grow ? exp2_fast(mx - m_new) : 1.f;
+      l *= alpha;
 #pragma unroll
-      for (int m = 0; m < MW; ++m) {
-        float pe = sc[m][0];
+      for (int dt = 0; dt < C::DT; ++dt) acc[dt] *= alpha;
+      mx = m_new;
+    }
+    const float neg_m = mx == -INFINITY ? 0.f : -mx;
 #pragma unroll
-        for (int e = 1; e < 16; ++e) pe = e == es ? sc[m][e] : pe;
-        pe = __shfl(pe, l32 + 32 * ((tk >> 2) & 1));
-        const bool seen = (vis[m] >> tk) & 1u;
+    for (int e4 = 0; e4 < 4; ++e4) {
+#pragma unroll
+      for (int kk = 0; kk < C::KK; ++kk)
+        if (kk * 4 / (C::KK < 4 ? 4 : C::KK) == e4) load_key(st_next, kk);  // (of the last tile: of no use)
+#pragma unroll
+      for (int e = 4 * e4; e < 4 * e4 + 4; ++e) sc[e] = exp2_fast(fmaf(sc[e], c, neg_m));
+      l += (sc[4 * e4] + sc[4 * e4 + 1]) + (sc[4 * e4 + 2] + sc[4 * e4 + 3]);
+      pb[e4 >> 1][2 * (e4 & 1)] = E::pack2(sc[4 * e4], sc[4 * e4 + 1]);
+      pb[e4 >> 1][2 * (e4 & 1) + 1] = E::pack2(sc[4 * e4 + 2], sc[4 * e4 + 3]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    st_prev = st_cur;
+    st_cur = st_next;
+  }
+
+  // ---- values that are not finite ----------------------------------------------
+  if (whole < T) {
+    __syncthreads();
+    for (int x = 0; x < T - whole; ++x)
+      for (uint32_t keys = odd[hh * kTreeOddWords + x]; keys; keys &= keys - 1) {
+        // the row's probability of that key once more, for the columns taken out
+        const int key = kPagedTile * (tlo + whole + x) + __builtin_ctz(keys), a = key - base;
+        if (key >= ctx) continue;  // (a copy of the last token)
+        const int blk = (int)fdiv((uint32_t)key, p.bsdiv), off = key - blk * p.block_size;
+        const int64_t id = max(sbt[blk - blk_lo], 0);
+        const uint16_t* krow = p.kc + id * p.ks0 + (int64_t)off * p.ks1 + (int64_t)kvh * p.ks2;
+        const uint16_t* vrow = p.vc + id * p.vs0 + (int64_t)off * p.vs1 + (int64_t)kvh * p.vs2;
+        float s = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < C::KK; ++kk) {
+          const f32x8 kv = widen8<DTYPE>(load16_clamped(krow + 16 * kk + 8 * hl)), qv = widen8<DTYPE>(qf[kk]);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) s = fmaf(kv[y], qv[y], s);
+        }
+        s = xhalf_sum(s) * c;
+        const bool seen = live && (a < 0 || (words[a >> 5] >> (a & 31)) & 1);
+        const float pe = exp2_fast(s - (mx == -INFINITY ? 0.f : mx));
 #pragma unroll
         for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
           for (int g4 = 0; g4 < 4; ++g4) {
             const int d = 32 * dt + 8 * g4 + 4 * hl;
-            if (D < 32 && d >= D) continue;
-            const u32x2 v4 = *reinterpret_cast<const u32x2*>(vrow + ((hh * C::S + (d >> 3)) ^ sw) * 8 + (d & 7));
+            const u32x2 v4 = *reinterpret_cast<const u32x2*>(vrow + min(d, D - 4));
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const uint32_t h = y & 1 ? v4[y >> 1] >> 16 : v4[y >> 1] & 0xffffu;
-              if (seen && (h & kExp<DTYPE>) == kExp<DTYPE>) acc[m][dt][4 * g4 + y] += pe * widen<DTYPE>(h);
+              const float add = pe * widen<DTYPE>(h);
+              acc[dt][4 * g4 + y] += (seen & ((h & kExp<DTYPE>) == kExp<DTYPE>)) ? add : 0.f;
             }
           }
       }
-    }
   }
 
   // ---- output ----------------------------------------------------------------
-#pragma unroll
-  for (int m = 0; m < MW; ++m) {
-    const float lt = xhalf_sum(l[m]);
-    if (!rv[m]) continue;
-    if (n == 1) {
-      if (!live[m]) {
-        tree_fill<D>(orow[m], hl, 0u);
-        continue;
-      }
-      const float inv = poison ? __builtin_nanf("") : 1.f / lt;
-#pragma unroll
-      for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-          const int d = 32 * dt + 8 * g4 + 4 * hl;
-          if (D >= 32 || d < D)
-            *reinterpret_cast<u32x2*>(orow[m] + d) =
-                u32x2{E::pack2(acc[m][dt][4 * g4] * inv, acc[m][dt][4 * g4 + 1] * inv),
-                      E::pack2(acc[m][dt][4 * g4 + 2] * inv, acc[m][dt][4 * g4 + 3] * inv)};
-        }
-    } else {
-      const int r = ((rt * QT + qt) * MW + m) * 32 + l32;
-      const int64_t slot = ((int64_t)j * p.Hk + kvh) * p.R + r;
-      const float pz = poison ? __builtin_nanf("") : 1.f;
-#pragma unroll
-      for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-          const int d = 32 * dt + 8 * g4 + 4 * hl;
-          if (D >= 32 || d < D)
-            *reinterpret_cast<float4*>(p.part + slot * D + d) =
-                float4{acc[m][dt][4 * g4] * pz, acc[m][dt][4 * g4 + 1] * pz, acc[m][dt][4 * g4 + 2] * pz,
-                       acc[m][dt][4 * g4 + 3] * pz};
-        }
-      if (hl == 0) p.ml[slot] = float2{mx[m] * pz, lt * pz};
+  const float lt = xhalf_sum(l);
+  if (!rv) return;
+  if (n == 1) {
+    uint16_t* const orow = out_row();
+    if (!live) {
+      tree_fill<D>(orow, hl, 0u);
+      return;
     }
+    const float inv = poison ? __builtin_nanf("") : 1.f / lt;
+#pragma unroll
+    for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const int d = 32 * dt + 8 * g4 + 4 * hl;
+        if (D >= 32 || d < D)
+          *reinterpret_cast<u32x2*>(orow + d) =
+              u32x2{E::pack2(acc[dt][4 * g4] * inv, acc[dt][4 * g4 + 1] * inv),
+                    E::pack2(acc[dt][4 * g4 + 2] * inv, acc[dt][4 * g4 + 3] * inv)};
+      }
+    return;
   }
+  // a partial state in lane order, 1 KiB a store: [row group][column group][lane][4]
+  const int64_t slot = ((int64_t)j * p.Hk + kvh) * p.G32 + (rt * QT + qt);
+  float* const part = p.part + slot * (32 * D) + 4 * lane;
+  const float pz = poison ? __builtin_nanf("") : 1.f;
+#pragma unroll
+  for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      if (D >= 32 || g4 < D / 8)
+        *reinterpret_cast<float4*>(part + 256 * (4 * dt + g4)) =
+            float4{acc[dt][4 * g4] * pz, acc[dt][4 * g4 + 1] * pz, acc[dt][4 * g4 + 2] * pz, acc[dt][4 * g4 + 3] * pz};
+  if (hl == 0) p.ml[slot * 32 + l32] = float2{mx * pz, lt * pz};
 }
 
 // Writes the nodes' K and V behind the history before attention reads them:
@@ -490,52 +527,51 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
   *reinterpret_cast<u32x4*>(vd + half) = v1;
 }
 
-// Combines the pieces of every sequence that has more than one. Eight lanes
-// share a row's four columns: lane t takes pieces t, t + 8, ..., then a fixed
-// butterfly joins the eight states.
-constexpr int kTreeMergeLanes = 8, kTreeMergeBatch = 4;
+// Combines the pieces of every sequence that has more than one: a workgroup
+// takes one column group (8 columns of 32 rows, 64 lanes x 4 values) and its
+// four waves the pieces in turn, each reading whole 1 KiB runs of the partial
+// states; the four results are joined in wave order.
+constexpr int kTreeMergeWaves = 4, kTreeMergeBatch = 4;
 
 template <int DTYPE, int D>
-__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p) {
+__global__ __launch_bounds__(64 * kTreeMergeWaves) void tree_merge_kernel(const TreeParams p) {
   using E = Elt<DTYPE>;
-  constexpr int Q4 = D / 4;
-  warm_kernargs<sizeof(TreeParams)>();
+  __shared__ float4 sa[kTreeMergeWaves][64];
+  __shared__ float2 sm[kTreeMergeWaves][64];
   const int b = blockIdx.y;
   const int2 inf = p.info[b];
   if (inf.y < 2) return;  // written whole by the main pass
-  const uint32_t tid = blockIdx.x * 256u + threadIdx.x;
-  const int t = (int)(tid % kTreeMergeLanes);
-  const uint32_t item = tid / kTreeMergeLanes;
-  const int d4 = (int)(item % Q4);
-  const uint32_t row = item / Q4;  // kvh * R + r
-  const bool in = row < (uint32_t)(p.Hk * p.R);
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hl = lane >> 5;
+  const int cg = blockIdx.x % (D / 8), rg = blockIdx.x / (D / 8);  // rg = kvh * G32 + row group
+  const int kvh = rg / p.G32, r = (rg - kvh * p.G32) * 32 + l32;
   float M = -INFINITY, L = 0.f;
   float4 A = {0.f, 0.f, 0.f, 0.f};
-  if (in)
-    for (int k0 = t; k0 < inf.y; k0 += kTreeMergeLanes * kTreeMergeBatch) {
+  if (r < p.R)
+    for (int k0 = w; k0 < inf.y; k0 += kTreeMergeWaves * kTreeMergeBatch) {
       float2 ml[kTreeMergeBatch];
       float4 a[kTreeMergeBatch];
 #pragma unroll
       for (int u = 0; u < kTreeMergeBatch; ++u) {
-        const int k = min(k0 + kTreeMergeLanes * u, inf.y - 1);
-        const int64_t slot = (int64_t)(inf.x + k) * p.Hk * p.R + row;
-        ml[u] = p.ml[slot];
-        a[u] = *reinterpret_cast<const float4*>(p.part + slot * D + 4 * d4);
+        const int k = min(k0 + kTreeMergeWaves * u, inf.y - 1);
+        const int64_t slot = (int64_t)(inf.x + k) * p.Hk * p.G32 + rg;
+        ml[u] = p.ml[slot * 32 + l32];
+        a[u] = *reinterpret_cast<const float4*>(p.part + slot * (32 * D) + 256 * cg + 4 * lane);
       }
 #pragma unroll
       for (int u = 0; u < kTreeMergeBatch; ++u)
-        if (k0 + kTreeMergeLanes * u < inf.y) merge_state(M, L, A, ml[u].x, ml[u].y, a[u]);
+        if (k0 + kTreeMergeWaves * u < inf.y) merge_state(M, L, A, ml[u].x, ml[u].y, a[u]);
     }
-  butterfly_step<1>(t, M, L, A);
-  butterfly_step<2>(t, M, L, A);
-  butterfly_step<4>(t, M, L, A);
-  if (!in || t != 0) return;
-  const int kvh = (int)(row / (uint32_t)p.R), r = (int)(row - (uint32_t)kvh * (uint32_t)p.R);
+  sa[w][lane] = A;
+  sm[w][lane] = float2{M, L};
+  __syncthreads();
+  if (w != 0 || r >= p.R) return;
+#pragma unroll
+  for (int x = 1; x < kTreeMergeWaves; ++x) merge_state(M, L, A, sm[x][lane].x, sm[x][lane].y, sa[x][lane]);
   const int g = (int)fdiv((uint32_t)r, p.ndiv), i = r - g * p.N;
   const bool live = tree_row_live(p.mask + (int64_t)b * p.ms0 + (int64_t)i * p.ms1, p.N);
   const float inv = 1.f / L;
   uint16_t* orow = p.o + (int64_t)b * p.os0 + (int64_t)(kvh * p.group + g) * p.os1 + (int64_t)i * p.os2;
-  *reinterpret_cast<u32x2*>(orow + 4 * d4) =
+  *reinterpret_cast<u32x2*>(orow + 8 * cg + 4 * hl) =
       live ? u32x2{E::pack2(A.x * inv, A.y * inv), E::pack2(A.z * inv, A.w * inv)} : u32x2{0u, 0u};
 }
 
@@ -551,41 +587,57 @@ TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int b
     return g;
   }
   const int64_t rows = (int64_t)(Hq / Hk) * N;
-  if (rows * Hk * (D / 4) * kTreeMergeLanes >= ((int64_t)1 << 31)) {
+  if (rows > 1 << 24) {
     g.err = "problem too large for one launch";
     return g;
   }
   g.R = (int)rows;
-  g.QT = g.R <= 32 ? 1 : g.R <= 64 ? 2 : 4;
-  g.MW = g.R > 128 && D <= 128 ? 2 : 1;
+  g.G32 = (g.R + 31) / 32;
+  g.QT = std::min(g.R <= 32 ? 1 : g.R <= 64 ? 2 : g.R <= 128 ? 4 : 8, D == 256 ? 4 : 8);
   g.HG = 1;
-  for (int h = 2; h <= 4 / g.QT; h *= 2)
+  for (int h = 2; h * g.QT * 64 <= tree_threads(D, g.QT); h *= 2)
     if (Hk % h == 0 && h * D <= 256) g.HG = h;
   g.NG = Hk / g.HG;
-  const int rt = 32 * g.QT * g.MW;
-  g.NRT = (g.R + rt - 1) / rt;
+  g.NRT = (g.R + 32 * g.QT - 1) / (32 * g.QT);
   g.NCH = g.HG * D / 8;
   const size_t stage = (size_t)2 * kPagedTile * g.NCH * 16;
-  g.NST = std::min(4, std::max(2, (int)((size_t)64 * 1024 / stage)));
+  // One workgroup per CU with a ring of 128 KiB, eight stages at most: 32 trees of 16
+  // nodes over 256-4096 tokens 40.5 us, 48 with 96 KiB (three 32 KiB stages), 48 and 41
+  // with two workgroups of 64 KiB and stages of 32 and 16.
+  g.NST = std::min(8, std::max(3, (int)((size_t)128 * 1024 / stage)));
   const int cpt = 2 * (D / (16 * std::min(g.QT, D / 16)));  // copies of an issuing wave per tile
-  g.NST = std::min(g.NST, 2 + 63 / cpt);                    // those of NST - 2 tiles in flight fit vmcnt
-  g.lds_bytes = (size_t)g.NST * stage;
-  const int wpc = std::max(1, std::min(2, (int)((size_t)150 * 1024 / (g.lds_bytes + sizeof(int32_t) * kTreeIds))));
+  g.NST = std::min(g.NST, 3 + 63 / cpt);                    // those of NST - 3 tiles in flight fit vmcnt
+  g.lds_bytes = (size_t)g.NST * stage + sizeof(int32_t) * (kTreeIds + g.HG * kTreeOddWords);
   const int64_t nt_max = (int64_t)B * ((ctx_limit + kPagedTile - 1) / kPagedTile);
   // tiles whose block ids the workgroup can stage
   const int64_t ccap = std::max<int64_t>(1, ((int64_t)(kTreeIds - 2) * block_size) / kPagedTile);
+  // Pieces beyond one per sequence: while the sequences' workgroups take at most half
+  // of the CUs, what fills them once, one workgroup per CU. Above, k per sequence,
+  // k the number whose last round of workgroups leaves the least idle (sequences
+  // longer than 1 / k of the average are cut too); a cut costs the partial states,
+  // taken as 4 % (48 sequences of one length, 32/8 heads, D = 128: k = 2).
   const int64_t per_piece = (int64_t)g.NG * g.NRT;
-  const int64_t want = ((int64_t)dev.cus * wpc + per_piece - 1) / per_piece;  // pieces that fill the device once
-  int64_t extra = std::max<int64_t>(std::max<int64_t>(want - B, want / 2), 1);
-  g.cmin = (int)std::min<int64_t>(ccap, g.R <= 64 ? 2 : 4);
+  int64_t extra = std::max<int64_t>(1, dev.cus / per_piece - B);
+  if (2 * B * per_piece > dev.cus) {
+    double least = 0;
+    for (int k = 1; k <= 4; ++k) {
+      const double rounds = (double)((k * B * per_piece + dev.cus - 1) / dev.cus) / k + 0.04 * (k - 1);
+      if (k == 1 || rounds < least) least = rounds, extra = k * B;
+    }
+  }
+  g.cmin = (int)std::min<int64_t>(ccap, 2);  // (one tile: 1 x 8 nodes over 777 tokens 12.0 -> 12.3 us; four: 13.5)
   extra = std::min(extra, std::max<int64_t>(1, (nt_max + g.cmin - 1) / g.cmin));
   extra = std::max(extra, (nt_max + ccap - 1) / ccap);
+  if (extra > INT_MAX / 2) {
+    g.err = "problem too large for one launch";
+    return g;
+  }
   g.extra = (int)extra;
   const int64_t pieces = B + extra;
   const int64_t units = pieces * g.NG;
   const int64_t nx = (int64_t)1 << dev.xcd_shift;
   const int64_t wgs = g.NRT > 1 ? (units + nx - 1) / nx * nx * g.NRT : units;
-  if (wgs > INT_MAX || B > 65535) {
+  if (wgs > INT_MAX || B > 65535 || (int64_t)Hk * g.G32 * (D / 8) > INT_MAX) {
     g.err = "problem too large for one launch";
     return g;
   }
@@ -593,7 +645,7 @@ TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int b
   // no sequence can have more than one piece when the longest has at most cmin tiles
   g.split = (ctx_limit + kPagedTile - 1) / kPagedTile > g.cmin;
   if (g.split) {
-    const size_t slots = (size_t)pieces * Hk * g.R;
+    const size_t slots = (size_t)pieces * Hk * g.G32 * 32;
     g.info_bytes = ((size_t)B * sizeof(int2) + 255) / 256 * 256;
     g.ml_bytes = (slots * sizeof(float2) + 255) / 256 * 256;
     g.part_bytes = slots * D * sizeof(float);
@@ -602,11 +654,11 @@ TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int b
   return g;
 }
 
-template <int DTYPE, int D, int QT, int MW>
+template <int DTYPE, int D, int QT>
 static hipError_t launch_tree_k(const TreeParams& p, const TreeGeom& g, hipStream_t stream) {
-  const hipError_t attr = set_dynamic_lds(reinterpret_cast<const void*>(&tree_fwd_kernel<DTYPE, D, QT, MW>), kPagedLdsBudget);
+  const hipError_t attr = set_dynamic_lds(reinterpret_cast<const void*>(&tree_fwd_kernel<DTYPE, D, QT>), kPagedLdsBudget);
   if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL((tree_fwd_kernel<DTYPE, D, QT, MW>), dim3((unsigned)g.wgs), dim3(64 * g.HG * QT), g.lds_bytes, stream, p);
+  hipLaunchKernelGGL((tree_fwd_kernel<DTYPE, D, QT>), dim3((unsigned)g.wgs), dim3(64 * g.HG * QT), g.lds_bytes, stream, p);
   return hipGetLastError();
 }
 
@@ -619,16 +671,16 @@ static hipError_t launch_tree_d(const TreeParams& p, const TreeGeom& g, hipStrea
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (g.QT == 1) e = launch_tree_k<DTYPE, D, 1, 1>(p, g, stream);
-  else if (g.QT == 2) e = launch_tree_k<DTYPE, D, 2, 1>(p, g, stream);
-  else if (g.MW == 1) e = launch_tree_k<DTYPE, D, 4, 1>(p, g, stream);
+  if (g.QT == 1) e = launch_tree_k<DTYPE, D, 1>(p, g, stream);
+  else if (g.QT == 2) e = launch_tree_k<DTYPE, D, 2>(p, g, stream);
+  else if (g.QT == 4) e = launch_tree_k<DTYPE, D, 4>(p, g, stream);
   else {
-    if constexpr (D <= 128) e = launch_tree_k<DTYPE, D, 4, 2>(p, g, stream);
+    if constexpr (D <= 128) e = launch_tree_k<DTYPE, D, 8>(p, g, stream);
     else return hipErrorInvalidValue;
   }
   if (e != hipSuccess || !g.split) return e;
-  const unsigned items = (unsigned)(p.Hk * p.R) * (D / 4) * kTreeMergeLanes;
-  hipLaunchKernelGGL((tree_merge_kernel<DTYPE, D>), dim3((items + 255) / 256, (unsigned)p.B), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((tree_merge_kernel<DTYPE, D>), dim3((unsigned)(p.Hk * p.G32 * (D / 8)), (unsigned)p.B),
+                     dim3(64 * kTreeMergeWaves), 0, stream, p);
   return hipGetLastError();
 }
 
