@@ -1103,7 +1103,7 @@ int cie_draft_masks(const int32_t* parents, int32_t* mask, int32_t* depths, uint
 static int verify_impl(const void* target, const void* draft, const void* draft_tokens, int token_bytes,
                        const int32_t* parents, const void* uniforms, int uniform_bytes, void* tokens, int32_t* path,
                        int32_t* counts, const int64_t* ts, const int64_t* ds, int B, int N, int V, int dtype, int mode,
-                       void* stream) {
+                       void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != CIE_TABLE_F16 && dtype != CIE_TABLE_BF16 && dtype != CIE_TABLE_F32)
     return fail(CIE_EDTYPE, "unsupported dtype code %d (f16 = 0, bf16 = 1, f32 = 2)", dtype);
   if (B < 0 || N < 0 || V < 0) return fail(CIE_EINVAL, "negative size (B=%d, N=%d, V=%d)", B, N, V);
@@ -1138,6 +1138,13 @@ static int verify_impl(const void* target, const void* draft, const void* draft_
   p.counts = counts;
   p.ts0 = ts[0]; p.ts1 = ts[1];
   if (mode > 0) p.ds0 = ds[0], p.ds1 = ds[1];
+  const size_t need = mode < 0 ? cie::verify_tops_bytes(B, N, V, dtype) : 0;
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail(CIE_EWORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    if (!aligned16(workspace)) return fail(CIE_EINVAL, "workspace: pointer is not 16-byte aligned");
+    p.tops = static_cast<uint64_t*>(workspace);
+  }
   p.token_bytes = token_bytes;
   p.uniform_bytes = uniform_bytes;
   p.B = B; p.N = N; p.V = V;
@@ -1152,14 +1159,20 @@ int cie_verify_draft(const void* target_probs, const void* draft_probs, const vo
                      int dtype, int replacement, void* stream) {
   return verify_impl(target_probs, draft_probs, draft_tokens, token_bytes, parents, uniforms, uniform_bytes, tokens,
                      path, counts, target_stride, draft_stride, B, N, V, dtype,
-                     !draft_probs ? 0 : replacement ? 1 : 2, stream);
+                     !draft_probs ? 0 : replacement ? 1 : 2, nullptr, 0, stream);
+}
+
+size_t cie_verify_greedy_workspace_bytes(int B, int N, int V, int dtype) {
+  if (B < 1 || N < 1 || N > cie::kTreeMaxNodes || V < 1 || V > (1 << 30) || dtype < CIE_TABLE_F16 || dtype > CIE_TABLE_F32)
+    return 0;
+  return cie::verify_tops_bytes(B, N, V, dtype);
 }
 
 int cie_verify_greedy(const void* target_logits, const void* draft_tokens, int token_bytes, const int32_t* parents,
                       void* tokens, int32_t* path, int32_t* counts, const int64_t* target_stride, int B, int N, int V,
-                      int dtype, void* stream) {
+                      int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   return verify_impl(target_logits, nullptr, draft_tokens, token_bytes, parents, nullptr, 0, tokens, path, counts,
-                     target_stride, nullptr, B, N, V, dtype, -1, stream);
+                     target_stride, nullptr, B, N, V, dtype, -1, workspace, workspace_bytes, stream);
 }
 
 int cie_kv_keep(void* const* k_caches, void* const* v_caches, int layers, const int64_t* k_stride,

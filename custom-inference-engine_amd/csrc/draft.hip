@@ -80,16 +80,17 @@ hipError_t launch_draft_masks(const int32_t* parents, int32_t* mask, int32_t* de
 // pass over the rows per rejection gives W (one per node for the draft's own
 // picks, whose W follows from the children's p), and none is needed before a
 // first rejection: each child's p(x), q(x) and u are fetched once for the whole
-// tree, one thread a node.
+// tree, one thread a node. A step down the tree costs 0.5 us then, the start and
+// the end 4 us, and the passes the rest.
 //
 // All sums are 64-bit: the last token is a comparison of a sum over the
 // vocabulary with u_0 times that sum, and has to come out the same whatever the
 // order of the summation; in 32 bits one draw in some thousands would not.
 //
-// One workgroup of 16 waves per sequence, each wave over a contiguous 16th of
-// the vocabulary, so that the wave holding the last token follows from the 16
-// wave sums and only its part is read again.
+// The vocabulary is cut into 64 parts at most whose sums are kept, so that the
+// part holding the last token follows from them and only it is read again.
 constexpr int kVerifyWaves = 16, kVerifyThreads = 64 * kVerifyWaves;
+constexpr int kParts = 64;
 constexpr double kNoMass = 0x1p-40;
 
 template <int DT> struct ProbElt;  // 0 fp16, 1 bf16, 2 fp32: 16 bytes a load, rows of any alignment
@@ -177,31 +178,41 @@ __device__ __forceinline__ void token_store(void* tokens, int bytes, int64_t i, 
 // either of them without the listed tokens; that residual and q without them.
 enum { kSumP, kSumPWithout, kSumRest, kSumRestWithout, kSumRestQWithout };
 
-// That sum over [lo, hi) by one wave, 16 bytes a lane and four loads of each
-// row in flight. The listed tokens (the children of the node) are left out
-// rather than subtracted later: what remains may be a small part of the sum.
+// Tokens of a part of the vocabulary: what one wave has in flight at once, or
+// more where 64 parts of that do not cover it.
+__device__ __forceinline__ int part_tokens(int V) {
+  constexpr int E = 64 * 32;
+  return ((V + kParts - 1) / kParts + E - 1) / E * E;
+}
+
+// Those sums for parts w, w + 16, .. of a row, by one wave, to psum[part] (and
+// that of q to pq[part]). The listed tokens (the children of the node) are left
+// out rather than subtracted later: what remains may be a small part of the sum.
+// Bound by what one CU has under way to memory: 78 GB/s, p alone or both rows
+// (128000 fp32 tokens: 6.6 and 13 us). The next block, of this part or the next,
+// is asked for before this one is summed; full parts go through a loop without
+// a branch around a load, the last one apart.
 template <int DT, int WHAT>
 __device__ __forceinline__ void wave_sums(const typename ProbElt<DT>::T* P, const typename ProbElt<DT>::T* Q, double c,
-                                          int lo, int hi, int lane, const int32_t* list, int nlist, double& sum,
-                                          double& qsum) {
+                                          int V, int w, int lane, const int32_t* list, int nlist, double* psum,
+                                          double* pq) {
   using E = ProbElt<DT>;
-  constexpr int U = 16 / E::V, BLOCK = 64 * E::V * U;
   constexpr bool REST = WHAT >= kSumRest, LIST = WHAT != kSumP && WHAT != kSumRest;
-  double s[2] = {0.0, 0.0}, sq = 0.0;
-  for (int at = lo; at < hi; at += BLOCK) {
+  constexpr int U = (DT == 2 || (REST && LIST) ? 16 : 32) / E::V, BLOCK = 64 * E::V * U;  // (two blocks in 128 registers)
+  struct Block {
     u32x4 a[U], q[U];
+  };
+  const int per = part_tokens(V), full = V / per, blocks = per / BLOCK;
+  double s[2] = {0.0, 0.0}, sq = 0.0;
+  auto load = [&](Block& x, int at) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int y = at + (64 * u + lane) * E::V;
-      a[u] = q[u] = u32x4{0u, 0u, 0u, 0u};
-      if (y + E::V <= hi) {
-        a[u] = E::load(P + y);
-        if (REST) q[u] = E::load(Q + y);
-      } else if (y < hi) {
-        a[u] = E::load_part(P + y, hi - y);
-        if (REST) q[u] = E::load_part(Q + y, hi - y);
-      }
+      x.a[u] = E::load(P + y);
+      if (REST) x.q[u] = E::load(Q + y);
     }
+  };
+  auto add = [&](Block& x, int at) {
     if (LIST)
       for (int g0 = 0; g0 < nlist; g0 += 64) {
         const int mine = g0 + lane < nlist ? list[g0 + lane] - at : -1;
@@ -211,8 +222,8 @@ __device__ __forceinline__ void wave_sums(const typename ProbElt<DT>::T* P, cons
 #pragma unroll
           for (int u = 0; u < U; ++u)
             if (own == 64 * u + lane) {
-              E::clear(a[u], rel % E::V);
-              if (REST) E::clear(q[u], rel % E::V);
+              E::clear(x.a[u], rel % E::V);
+              if (REST) E::clear(x.q[u], rel % E::V);
             }
         }
       }
@@ -220,33 +231,86 @@ __device__ __forceinline__ void wave_sums(const typename ProbElt<DT>::T* P, cons
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < E::V; ++e) {
-        const double pp = (double)E::get(a[u], e);
+        const double pp = (double)E::get(x.a[u], e);
         if (REST) {
-          const double qq = (double)E::get(q[u], e);
+          const double qq = (double)E::get(x.q[u], e);
           s[e & 1] += __builtin_fmax(__builtin_fma(-c, qq, pp), 0.0);
           if (WHAT == kSumRestQWithout) sq += qq;
         } else {
           s[e & 1] += pp;
         }
       }
+  };
+  auto finish = [&](int part) {
+    const double sum = wave_sum(s[0] + s[1]);
+    const double qsum = WHAT == kSumRestQWithout ? wave_sum(sq) : 0.0;
+    if (lane == 0) psum[part] = sum;
+    if (WHAT == kSumRestQWithout && lane == 0) pq[part] = qsum;
+    s[0] = s[1] = sq = 0.0;
+  };
+  if (w < full) {
+    Block now, next;
+    int part = w, k = 0;
+    load(now, part * per);
+    for (;;) {
+      const int at = part * per + k * BLOCK;
+      const bool ends = k + 1 == blocks;
+      const int part2 = ends ? part + kVerifyWaves : part, k2 = ends ? 0 : k + 1;
+      if (part2 >= full) break;
+      load(next, part2 * per + k2 * BLOCK);
+      add(now, at);
+      if (ends) finish(part);
+      now = next;
+      part = part2, k = k2;
+    }
+    add(now, part * per + k * BLOCK);
+    finish(part);
   }
-  sum = wave_sum(s[0] + s[1]);
-  if (WHAT == kSumRestQWithout) qsum = wave_sum(sq);
+  if (full * per < V && (full & (kVerifyWaves - 1)) == w) {
+    for (int at = full * per; at < V; at += BLOCK) {
+      Block x;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int y = at + (64 * u + lane) * E::V;
+        x.a[u] = x.q[u] = u32x4{0u, 0u, 0u, 0u};
+        if (y + E::V <= V) {
+          x.a[u] = E::load(P + y);
+          if (REST) x.q[u] = E::load(Q + y);
+        } else if (y < V) {
+          x.a[u] = E::load_part(P + y, V - y);
+          if (REST) x.q[u] = E::load_part(Q + y, V - y);
+        }
+      }
+      add(x, at);
+    }
+    finish(full);
+  }
 }
 
 enum { kDraftPicks = 0, kDraftIid = 1, kDraftTree = 2 };
+
+// A tree's parents and tokens as the kernels use them: a node that can never be
+// tried (a padding slot, a parent that does not come before it, a token outside
+// the vocabulary) has parent -2.
+__device__ __forceinline__ void tree_node(const VerifyParams& p, int b, int i, int& up, int& x) {
+  up = p.parents[(int64_t)b * p.N + i];
+  const int64_t t = token_at(p.draft_tokens, p.token_bytes, (int64_t)b * p.N + i);
+  const bool known = t >= 0 && t < p.V;
+  x = known ? (int)t : -1;
+  if (i > 0 && !(up >= 0 && up < i && known)) up = -2;
+}
 
 template <int DT, int MODE>
 __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const VerifyParams p) {
   using E = ProbElt<DT>;
   using T = typename E::T;
   __shared__ int32_t par[kTreeMaxNodes], tok[kTreeMaxNodes], path[kTreeMaxNodes];
-  __shared__ int32_t list[kTreeMaxNodes];           // the distinct tokens of the node's children
+  __shared__ int32_t list[kTreeMaxNodes];                  // the distinct tokens of the node's children
   __shared__ uint8_t out_of[kVerifyWaves][kTreeMaxNodes];  // which of them are out, each wave's own copy
   __shared__ float pg[kTreeMaxNodes], qg[kTreeMaxNodes], lp[kTreeMaxNodes], lq[kTreeMaxNodes];
   __shared__ double kept[kTreeMaxNodes];  // drafts without replacement: what p has left of a token that q lost
   __shared__ double ug[kTreeMaxNodes];
-  __shared__ double wsum[2][kVerifyWaves], wq[kVerifyWaves], wpre[kVerifyWaves];
+  __shared__ double psum[2][kParts], pq[kParts], wpre[kVerifyWaves];
   __shared__ int found, lastpos;
   const int b = blockIdx.x, i = threadIdx.x, lane = i & 63;
   const int w = __builtin_amdgcn_readfirstlane(i >> 6);
@@ -254,11 +318,11 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
   const T* const target = static_cast<const T*>(p.target) + (int64_t)b * p.ts0;
   const T* const draft = MODE == kDraftPicks ? nullptr : static_cast<const T*>(p.draft) + (int64_t)b * p.ds0;
   if (i < N) {
-    const int up = p.parents[(int64_t)b * N + i];
-    const int64_t x = token_at(p.draft_tokens, p.token_bytes, (int64_t)b * N + i);
-    const bool child = up >= 0 && up < i && x >= 0 && x < V;  // others are never tried
-    par[i] = i == 0 ? up : child ? up : -2;
-    tok[i] = child ? (int)x : -1;
+    int up, x;
+    tree_node(p, b, i, up, x);
+    const bool child = i > 0 && up >= 0;
+    par[i] = up;
+    tok[i] = x;
     pg[i] = child ? E::at(target + (int64_t)up * p.ts1 + x) : 0.f;
     qg[i] = child && MODE != kDraftPicks ? E::at(draft + (int64_t)up * p.ds1 + x) : 1.f;
     ug[i] = p.uniform_bytes == 8 ? static_cast<const double*>(p.uniforms)[(int64_t)b * N + i]
@@ -270,38 +334,43 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
   int cur = 0, count = active ? 1 : 0;
   int64_t last = -1;
   if (active) {
-    // this wave's part of the vocabulary
-    const int per = ((V + kVerifyWaves - 1) / kVerifyWaves + E::V - 1) / E::V * E::V;
-    const int lo = min(w * per, V), hi = min(lo + per, V);
+    const int per = part_tokens(V), parts = (V + per - 1) / per;
     const T *P = nullptr, *Q = nullptr;
-    int buf = 0;   // wsum[buf] holds the wave sums of the current residual when `have`
+    int buf = 0;   // psum[buf] holds the sums of the current residual's parts when `have`
     int nlist = 0;
     bool have = false;
     double qlist = 0.0;  // sum of q without the listed tokens
-    // one pass; the wave sums go to wsum[buf ^ 1], the total is the same on every thread
+    // One pass over the row. The parts' sums go to psum[buf ^ 1], the total is the
+    // same on every thread.
     auto scan = [&](auto what, double cc) {
       constexpr int WHAT = decltype(what)::value;
-      double s, q = 0.0;
-      wave_sums<DT, WHAT>(P, Q, cc, lo, hi, lane, list, nlist, s, q);
-      if (lane == 0) wsum[buf ^ 1][w] = s, wq[w] = q;
+      wave_sums<DT, WHAT>(P, Q, cc, V, w, lane, list, nlist, psum[buf ^ 1], pq);
       __syncthreads();
-      double t = 0.0, tq = 0.0;
-      for (int x = 0; x < kVerifyWaves; ++x) t += wsum[buf ^ 1][x], tq += wq[x];
-      if (WHAT == kSumRestQWithout) qlist = tq;
-      __syncthreads();  // wq and the other buffer may be written again
+      const double t = wave_sum(lane < parts ? psum[buf ^ 1][lane] : 0.0);
+      if (WHAT == kSumRestQWithout) qlist = wave_sum(lane < parts ? pq[lane] : 0.0);
+      __syncthreads();  // pq and the other buffer may be written again
       return t;
     };
     uint8_t* const gone = out_of[w];
     double W, c, S, total, rest = 0.0;
-    // p's residual at listed token g for the scalar cc, and q there
+    // p's residual at listed token g for the scalar cc
     auto rest_of = [&](int g, double cc) {
       if (MODE == kDraftPicks) return gone[g] ? 0.0 : (double)lp[g];
       return gone[g] ? kept[g] : __builtin_fmax(__builtin_fma(-cc, (double)lq[g], (double)lp[g]), 0.0);
     };
-    auto list_rest = [&](double cc) {
+    // the sum of f over the list, on every lane
+    auto over_list = [&](auto f) {
       double t = 0.0;
-      for (int g = 0; g < nlist; ++g) t += rest_of(g, cc);
-      return t;
+      for (int g = lane; g < nlist; g += 64) t += f(g);
+      return wave_sum(t);
+    };
+    // a token's place in the list, or -1
+    auto place = [&](int x) {
+      for (int g0 = 0; g0 < nlist; g0 += 64) {
+        const uint64_t m = __builtin_amdgcn_ballot_w64(g0 + lane < nlist && list[g0 + lane] == x);
+        if (m) return g0 + (int)__builtin_ctzll(m);
+      }
+      return -1;
     };
     for (;;) {
       P = target + (int64_t)cur * p.ts1;
@@ -311,9 +380,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
       int taken = -1;
       for (int ch = next_child(par, N, cur, cur, lane); ch >= 0; ch = next_child(par, N, cur, ch, lane)) {
         const int x = tok[ch];
-        int at = -1;  // the token's place in the list
-        if (MODE != kDraftIid)
-          for (int g = 0; g < nlist; ++g) at = list[g] == x ? g : at;
+        int at = MODE == kDraftIid ? -1 : place(x);
         const bool out = at >= 0 && gone[at];  // out of p (picks) or of q (no replacement)
         const double qx = (double)qg[ch];
         const double r = at >= 0                ? rest_of(at, c)
@@ -328,9 +395,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
           // (every wave writes the same list; none still reads the one before)
           __syncthreads();
           for (int k = ch; k >= 0; k = next_child(par, N, cur, k, lane)) {
-            bool known = false;
-            for (int g = 0; g < nlist; ++g) known |= list[g] == tok[k];
-            if (known) continue;
+            if (place(tok[k]) >= 0) continue;
             list[nlist] = tok[k];
             lp[nlist] = pg[k];
             lq[nlist] = qg[k];
@@ -344,19 +409,20 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
             rest = scan(std::integral_constant<int, kSumPWithout>{}, 0.0);
             buf ^= 1;
             have = true;
-            total = rest + list_rest(0.0);
+            total = rest + over_list([&](int g) { return rest_of(g, 0.0); });
           }
           const bool was = gone[at];
           gone[at] = 1;
-          const double t = rest + list_rest(0.0);
+          const double t = rest + over_list([&](int g) { return rest_of(g, 0.0); });
           if (t / W > kNoMass) W = total = t;
           else gone[at] = was;
         } else {
           const double c2 = c + W / S;
           double t;
           if (MODE == kDraftIid) t = scan(std::integral_constant<int, kSumRest>{}, c2);
-          else if (first) t = scan(std::integral_constant<int, kSumRestQWithout>{}, c2) + list_rest(c2);
-          else t = scan(std::integral_constant<int, kSumRestWithout>{}, c2) + list_rest(c2);
+          else if (first) t = scan(std::integral_constant<int, kSumRestQWithout>{}, c2);
+          else t = scan(std::integral_constant<int, kSumRestWithout>{}, c2);
+          if (MODE == kDraftTree) t += over_list([&](int g) { return rest_of(g, c2); });
           if (t / W > kNoMass) {
             c = c2;
             W = total = t;
@@ -365,8 +431,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
           }
           if (MODE == kDraftTree && !out) {
             gone[at] = 1;
-            double m = qlist;
-            for (int g = 0; g < nlist; ++g) m += gone[g] ? 0.0 : (double)lq[g];
+            const double m = qlist + over_list([&](int g) { return gone[g] ? 0.0 : (double)lq[g]; });
             if (m / S > kNoMass) {
               S = m;
               kept[at] = __builtin_fmax(__builtin_fma(-c, qx, (double)pg[ch]), 0.0);
@@ -387,24 +452,29 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
       total = scan(std::integral_constant<int, kSumP>{}, 0.0);
       buf ^= 1;
     }
-    // the wave part that the last token lies in, then the token
+    // the part that the last token lies in (the same on every wave)
     const double goal = ug[0] * total;
-    double before = 0.0, s = 0.0;
-    int part = -1;
-    for (int x = 0; x < kVerifyWaves; ++x) {
-      double sx = wsum[buf][x];
-      if (MODE != kDraftIid)
-        for (int g = 0; g < nlist; ++g) sx += list[g] / per == x ? rest_of(g, c) : 0.0;
-      if (!(sx > 0.0)) continue;
-      if (part >= 0) before += s;
-      part = x, s = sx;
-      if (before + s > goal) break;
+    double mine = lane < parts ? psum[buf][lane] : 0.0;
+    if (MODE != kDraftIid)
+      for (int g = 0; g < nlist; ++g) {
+        const int at = list[g] - lane * per;
+        if (at >= 0 && at < per) mine += rest_of(g, c);
+      }
+    double incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double up = __shfl_up(incl, o);
+      if (lane >= o) incl += up;
     }
+    const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0.0);
+    const uint64_t over = __builtin_amdgcn_ballot_w64(mine > 0.0 && incl > goal);
+    const int part = over ? (int)__builtin_ctzll(over) : some ? 63 - (int)__builtin_clzll(some) : -1;
+    double before = __shfl(incl - mine, max(part, 0));
     // (from here nothing writes the list, and every wave's copy of `gone` says the same)
     const int plo = min(max(part, 0) * per, V), phi = part < 0 ? plo : min(plo + per, V);
-    constexpr int R = 8;  // tokens of a thread at once
+    constexpr int R = 2;  // tokens of a thread at once
     for (int at = plo; at < phi; at += R * kVerifyThreads) {
-      double r[R], mine = 0.0;
+      double r[R], sum = 0.0;
 #pragma unroll
       for (int e = 0; e < R; ++e) {
         const int y = at + R * i + e;
@@ -419,19 +489,19 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
 #pragma unroll
           for (int e = 0; e < R; ++e) r[e] = list[g] == at + R * i + e ? rest_of(g, c) : r[e];
 #pragma unroll
-      for (int e = 0; e < R; ++e) mine += r[e];
-      double incl = mine;
+      for (int e = 0; e < R; ++e) sum += r[e];
+      double upto = sum;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(incl, o);
-        if (lane >= o) incl += up;
+        const double up = __shfl_up(upto, o);
+        if (lane >= o) upto += up;
       }
-      if (lane == 63) wpre[w] = incl;
+      if (lane == 63) wpre[w] = upto;
       __syncthreads();
-      double run = before + (incl - mine), sum = 0.0;
+      double run = before + (upto - sum);
       for (int x = 0; x < kVerifyWaves; ++x) {
         if (x < w) run += wpre[x];
-        sum += wpre[x];
+        before += wpre[x];
       }
       int hit = V, pos = -1;
 #pragma unroll
@@ -442,9 +512,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
         run += r[e];
         if (r[e] > 0.0 && run > goal && hit == V) hit = at + R * i + e;
       }
-      if (hit < V) atomicMin(&found, hit);
-      if (pos >= 0) atomicMax(&lastpos, pos);
-      before += sum;
+      // (one atomic a wave: 64 on one word take the LDS 64 turns)
+      const uint64_t hits = __builtin_amdgcn_ballot_w64(hit < V), any = __builtin_amdgcn_ballot_w64(pos >= 0);
+      if (hits && lane == (int)__builtin_ctzll(hits)) atomicMin(&found, hit);
+      if (any && lane == 63 - (int)__builtin_clzll(any)) atomicMax(&lastpos, pos);
       __syncthreads();
       if (found < V) break;
     }
@@ -469,64 +540,105 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// An entry as one comparable number: its key, then the complement of its index.
+__device__ __forceinline__ uint64_t logit_entry(float x, int y) { return (uint64_t)logit_key(x) << 32 | (uint32_t)~y; }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t wave_largest(uint64_t top) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) top = larger(top, (uint64_t)__shfl_xor((unsigned long long)top, o));
+  return top;
+}
+
+// The largest entry of [lo, hi) of a row, hi > lo, among threads i, i + n, .. of
+// n. A lane keeps its largest value (NaN wins, the first one) and the 16 bytes
+// it stood in, two instructions an entry, and looks for the place in them at the
+// end. Addresses past the last 16 bytes are moved back to them: what is seen
+// twice changes nothing.
+template <int DT>
+__device__ __forceinline__ uint64_t largest_of(const typename ProbElt<DT>::T* P, int lo, int hi, int i, int n) {
+  using E = ProbElt<DT>;
+  constexpr int U = 8;
+  if (hi - lo < E::V) return lo + i < hi ? logit_entry(E::at(P + lo + i), lo + i) : 0;
+  float top = -__builtin_inff();
+  int where = min(lo + i * E::V, hi - E::V);
+  for (int at = lo; at < hi; at += n * E::V * U) {
+    u32x4 a[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) a[u] = E::load(P + min(at + (n * u + i) * E::V, hi - E::V));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float m = E::get(a[u], 0);
+#pragma unroll
+      for (int e = 1; e < E::V; ++e) m = __builtin_elementwise_maximum(m, E::get(a[u], e));
+      const bool more = top == top && !(m <= top);
+      top = more ? m : top;
+      where = more ? min(at + (n * u + i) * E::V, hi - E::V) : where;
+    }
+  }
+  const u32x4 a = E::load(P + where);
+  int y = 0;
+#pragma unroll
+  for (int e = E::V - 1; e >= 0; --e) {
+    const float x = E::get(a, e);
+    if (x == top || (x != x && top != top)) y = where + e;
+  }
+  return logit_entry(top, y);
+}
+
+// The largest entry of every part of every row of every tree, a wave each.
+// Bound by the bytes of the logits.
+constexpr int kTopParts = 16;
+template <int DT>
+__global__ __launch_bounds__(256) void verify_tops_kernel(const VerifyParams p) {
+  using T = typename ProbElt<DT>::T;
+  constexpr int E = 64 * ProbElt<DT>::V;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int s = (int)(unit % kTopParts);
+  const int64_t row = unit / kTopParts;
+  const int b = (int)(row / p.N), node = (int)(row - (int64_t)b * p.N);  // (16 units a row: no workgroup hangs over)
+  int own, unused;
+  tree_node(p, b, node, own, unused);
+  if (own < -1) return;  // no walk gets there
+  const int per = ((p.V + kTopParts - 1) / kTopParts + E - 1) / E * E;
+  const int lo = min(s * per, p.V), hi = min(lo + per, p.V);
+  const T* const P = static_cast<const T*>(p.target) + (int64_t)b * p.ts0 + (int64_t)node * p.ts1;
+  const uint64_t top = lo < hi ? wave_largest(largest_of<DT>(P, lo, hi, lane, 64)) : 0;
+  if (lane == 0) p.tops[unit] = top;
+}
+
 template <int DT>
 __global__ __launch_bounds__(kVerifyThreads) void verify_greedy_kernel(const VerifyParams p) {
-  using E = ProbElt<DT>;
-  using T = typename E::T;
-  __shared__ int32_t par[kTreeMaxNodes], tok[kTreeMaxNodes], path[kTreeMaxNodes];
-  __shared__ uint64_t best[2][kVerifyWaves];
+  using T = typename ProbElt<DT>::T;
+  __shared__ int32_t par[kTreeMaxNodes], tok[kTreeMaxNodes], path[kTreeMaxNodes], best[kTreeMaxNodes];
+  __shared__ uint64_t tops[2][kVerifyWaves];
   const int b = blockIdx.x, i = threadIdx.x, lane = i & 63;
   const int w = __builtin_amdgcn_readfirstlane(i >> 6);
-  const int N = p.N, V = p.V;
+  const int N = p.N;
   const T* const target = static_cast<const T*>(p.target) + (int64_t)b * p.ts0;
-  if (i < N) {
-    const int up = p.parents[(int64_t)b * N + i];
-    const int64_t x = token_at(p.draft_tokens, p.token_bytes, (int64_t)b * N + i);
-    par[i] = i == 0 ? up : up >= 0 && up < i && x >= 0 && x < V ? up : -2;
-    tok[i] = x >= 0 && x < V ? (int)x : -1;
+  if (i < N) tree_node(p, b, i, par[i], tok[i]);
+  if (p.tops && i < N) {
+    uint64_t top = 0;
+#pragma unroll
+    for (int x = 0; x < kTopParts; ++x) top = larger(top, p.tops[((int64_t)b * N + i) * kTopParts + x]);
+    best[i] = (int)~(uint32_t)top;
   }
   __syncthreads();
   const bool active = par[0] == -1;
   int cur = 0, count = active ? 1 : 0, buf = 0;
   int64_t last = -1;
   while (active) {
-    const T* P = target + (int64_t)cur * p.ts1;
-    // key high, complement of the index low: the largest is the first of the largest
-    uint64_t top = 0;
-    auto take = [&](float x, int y) {
-      const uint64_t k = (uint64_t)logit_key(x) << 32 | (uint32_t)~y;
-      top = k > top ? k : top;
-    };
-    constexpr int U = 16 / E::V;
-    for (int at = 0; at < V; at += kVerifyThreads * E::V * U) {
-      u32x4 a[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int y = at + (kVerifyThreads * u + i) * E::V;
-        a[u] = u32x4{0u, 0u, 0u, 0u};
-        if (y + E::V <= V) a[u] = E::load(P + y);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int y = at + (kVerifyThreads * u + i) * E::V;
-        if (y + E::V <= V) {
-#pragma unroll
-          for (int e = 0; e < E::V; ++e) take(E::get(a[u], e), y + e);
-        } else {
-          for (int z = y; z < V; ++z) take(E::at(P + z), z);
-        }
-      }
+    int t;
+    if (p.tops) {
+      t = best[cur];
+    } else {
+      uint64_t top = wave_largest(largest_of<DT>(target + (int64_t)cur * p.ts1, 0, p.V, i, kVerifyThreads));
+      if (lane == 0) tops[buf][w] = top;
+      __syncthreads();
+      for (int x = 0; x < kVerifyWaves; ++x) top = larger(top, tops[buf][x]);
+      buf ^= 1;  // (the next node's do not overwrite what another wave still reads)
+      t = (int)~(uint32_t)top;
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-      const uint64_t k = (uint64_t)__shfl_xor((unsigned long long)top, o);
-      top = k > top ? k : top;
-    }
-    if (lane == 0) best[buf][w] = top;
-    __syncthreads();
-    for (int x = 0; x < kVerifyWaves; ++x) top = best[buf][x] > top ? best[buf][x] : top;
-    buf ^= 1;  // (the next node's keys do not overwrite what another wave still reads)
-    const int t = (int)~(uint32_t)top;
     int ch = next_child(par, N, cur, cur, lane);
     while (ch >= 0 && tok[ch] != t) ch = next_child(par, N, cur, ch, lane);
     if (ch < 0) {
@@ -546,13 +658,31 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_greedy_kernel(const Ver
   if (i == 0) p.counts[b] = count;
 }
 
+// All rows first or one after another on the walk? The first costs the bytes of
+// the logits at 4.3 TB/s and a launch, whatever is accepted; the second 3 to 5 us
+// a visited node, whose row one CU reads at some 80 GB/s. Measured, bf16 (us,
+// rows first / on the walk, 2 to 5 nodes visited): 128000 tokens, 1 x 26
+// 12.9 / 25.2, 8 x 26 16.9 / 26.7, 16 x 26 (106 MB) 26.5 / 28.2, 32 x 26
+// 46.0 / 28.8; 32000 tokens, 1 x 8 12.5 / 13.2, 64 x 8 (33 MB) 13.9 / 16.3,
+// 64 x 26 (106 MB) 26.9 / 20.2.
+size_t verify_tops_bytes(int B, int N, int V, int dtype) {
+  const int64_t rows = (int64_t)B * N;
+  if (rows > (64ll << 20) / ((int64_t)V * (dtype == 2 ? 4 : 2))) return 0;
+  return (size_t)rows * kTopParts * sizeof(uint64_t);
+}
+
 template <int DT>
 static void launch_verify_t(const VerifyParams& p, int mode, hipStream_t stream) {
   const dim3 grid((unsigned)p.B), block(kVerifyThreads);
-  if (mode < 0) hipLaunchKernelGGL((verify_greedy_kernel<DT>), grid, block, 0, stream, p);
-  else if (mode == kDraftPicks) hipLaunchKernelGGL((verify_draft_kernel<DT, kDraftPicks>), grid, block, 0, stream, p);
+  if (mode == kDraftPicks) hipLaunchKernelGGL((verify_draft_kernel<DT, kDraftPicks>), grid, block, 0, stream, p);
   else if (mode == kDraftIid) hipLaunchKernelGGL((verify_draft_kernel<DT, kDraftIid>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((verify_draft_kernel<DT, kDraftTree>), grid, block, 0, stream, p);
+  else if (mode == kDraftTree) hipLaunchKernelGGL((verify_draft_kernel<DT, kDraftTree>), grid, block, 0, stream, p);
+  else {
+    if (p.tops)
+      hipLaunchKernelGGL((verify_tops_kernel<DT>), dim3((unsigned)((int64_t)p.B * p.N * kTopParts / 4)), dim3(256), 0,
+                         stream, p);
+    hipLaunchKernelGGL((verify_greedy_kernel<DT>), grid, block, 0, stream, p);
+  }
 }
 
 hipError_t launch_verify(const VerifyParams& p, int mode, int dtype, hipStream_t stream) {

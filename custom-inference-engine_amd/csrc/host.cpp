@@ -51,6 +51,7 @@ struct Api {
   decltype(&cie_tree_workspace_bytes) tree_ws;
   decltype(&cie_tree_attn) tree;
   decltype(&cie_verify_draft) verify;
+  decltype(&cie_verify_greedy_workspace_bytes) greedy_ws;
   decltype(&cie_verify_greedy) greedy;
   decltype(&cie_kv_keep) keep;
 } api;
@@ -58,7 +59,7 @@ const char* const kNames[] = {"cie_flash_workspace_bytes", "cie_flash_fwd_ex", "
                               "cie_flash_paged", "cie_paged_workspace_bytes", "cie_paged_fwd_ex", "cie_kv_append",
                               "cie_kv_append_rope", "cie_kv_append_seq", "cie_kv_gather", "cie_int8_matmul_workspace_bytes", "cie_int8_matmul",
                               "cie_draft_masks", "cie_tree_workspace_bytes", "cie_tree_attn", "cie_verify_draft",
-                              "cie_verify_greedy", "cie_kv_keep"};
+                              "cie_verify_greedy_workspace_bytes", "cie_verify_greedy", "cie_kv_keep"};
 constexpr size_t kFns = sizeof(kNames) / sizeof(kNames[0]);
 static_assert(sizeof(Api) == kFns * sizeof(void*), "one name per function, in order");
 
@@ -704,11 +705,13 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Strides st(*t), sd(d ? *d : *t);
   const int tb = (int)xc.element_size();
   int32_t *const pp = static_cast<int32_t*>(path.data_ptr()), *const cp = static_cast<int32_t*>(counts.data_ptr());
+  const size_t nbytes = u ? 0 : api.greedy_ws((int)B, (int)N, (int)V, any_code(*t));
+  const Tensor ws = nbytes ? bytes_like(nbytes, *t) : Tensor();
   void* stream = stream_of(*t);
   const int rc = launch([&] {
     if (!u)
       return api.greedy(t->data_ptr(), xc.data_ptr(), tb, ip(pc), tokens.data_ptr(), pp, cp, st.s, (int)B, (int)N,
-                        (int)V, any_code(*t), stream);
+                        (int)V, any_code(*t), nbytes ? ws.data_ptr() : nullptr, nbytes, stream);
     return api.verify(t->data_ptr(), d ? d->data_ptr() : nullptr, xc.data_ptr(), tb, ip(pc), uc.data_ptr(),
                       (int)uc.element_size(), tokens.data_ptr(), pp, cp, st.s, sd.s, (int)B, (int)N, (int)V,
                       any_code(*t), replacement, stream);

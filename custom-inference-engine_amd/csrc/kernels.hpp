@@ -296,12 +296,15 @@ struct VerifyParams {
   void* tokens;              // [B][N] like draft_tokens
   int32_t* path;             // [B][N]
   int32_t* counts;           // [B]
+  uint64_t* tops;            // greedy: the largest entries of every row's parts, or nullptr: the walk reads its rows
   int64_t ts0, ts1, ds0, ds1;
   int token_bytes, uniform_bytes;
   int B, N, V;
 };
 // mode: -1 greedy, 0 the draft's own picks, 1 drafts with replacement, 2 without; dtype as CIE_TABLE_*
 hipError_t launch_verify(const VerifyParams& p, int mode, int dtype, hipStream_t stream);
+// Bytes of `tops` for a greedy call, 0 when the walk is to read its rows itself.
+size_t verify_tops_bytes(int B, int N, int V, int dtype);
 
 constexpr int kKeepLayers = 64;  // layers of one launch (1 KiB of arguments)
 struct KeepParams {

@@ -59,6 +59,7 @@ EXPORTED_SYMBOLS = (
     "cie_tree_workspace_bytes",
     "cie_tree_attn",
     "cie_verify_draft",
+    "cie_verify_greedy_workspace_bytes",
     "cie_verify_greedy",
     "cie_kv_keep",
     "cie_int8_matmul_workspace_bytes",
@@ -164,7 +165,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cie_verify_draft.argtypes = [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i64p, _i64p,
                                      _i, _i, _i, _i, _i, _vp]
     lib.cie_verify_draft.restype = _i
-    lib.cie_verify_greedy.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i64p, _i, _i, _i, _i, _vp]
+    lib.cie_verify_greedy_workspace_bytes.argtypes = [_i] * 4
+    lib.cie_verify_greedy_workspace_bytes.restype = ctypes.c_size_t
+    lib.cie_verify_greedy.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i64p, _i, _i, _i, _i, _vp, ctypes.c_size_t, _vp]
     lib.cie_verify_greedy.restype = _i
     lib.cie_kv_keep.argtypes = [ctypes.POINTER(_vp), ctypes.POINTER(_vp), _i, _i64p, _i64p, _vp, _vp, _vp,
                                 ctypes.c_int64, _vp, _i, _i, _i, ctypes.c_int64, _i, _i, _i, _vp]

@@ -131,7 +131,10 @@ def _verify(name: str, target: torch.Tensor, draft_tokens: torch.Tensor, parents
     with torch.cuda.device(target.device):
         stream = _lib.stream_handle(target.device)
         if uniforms is None:
-            rc = lib.cie_verify_greedy(target.data_ptr(), *head, *outs, *sizes, stream)
+            nbytes = int(lib.cie_verify_greedy_workspace_bytes(*sizes))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=target.device) if nbytes else None
+            rc = lib.cie_verify_greedy(target.data_ptr(), *head, *outs, *sizes,
+                                       ws.data_ptr() if ws is not None else None, nbytes, stream)
         else:
             u = uniforms.contiguous()
             rc = lib.cie_verify_draft(target.data_ptr(), draft.data_ptr() if draft is not None else None, *head,

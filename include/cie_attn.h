@@ -565,15 +565,20 @@ int cie_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_c
  * Only the rows of the visited nodes are read. cie_verify_greedy: a child is
  * accepted iff its token is the largest of target_logits at its parent (the
  * lowest index of equal ones, a NaN the largest), which is also the last token.
+ * Its workspace: cie_verify_greedy_workspace_bytes bytes, 16-byte aligned, any
+ * contents, not shared by concurrent calls; 0 bytes (NULL allowed) when the rows
+ * are to be read one after another as the walk comes to them, which is chosen
+ * for large batches.
  * Reference: engine/decode/speculative.py:88-133 (greedy, one chain).
  */
+size_t cie_verify_greedy_workspace_bytes(int B, int N, int V, int dtype);
 int cie_verify_draft(const void* target_probs, const void* draft_probs, const void* draft_tokens, int token_bytes,
                      const int32_t* parents, const void* uniforms, int uniform_bytes, void* tokens, int32_t* path,
                      int32_t* counts, const int64_t* target_stride, const int64_t* draft_stride, int B, int N, int V,
                      int dtype, int replacement, void* stream);
 int cie_verify_greedy(const void* target_logits, const void* draft_tokens, int token_bytes, const int32_t* parents,
                       void* tokens, int32_t* path, int32_t* counts, const int64_t* target_stride, int B, int N, int V,
-                      int dtype, void* stream);
+                      int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Moves the K and V of the accepted path behind the history, in every layer:

@@ -218,6 +218,50 @@ def test_greedy_ties_infinities_and_nan():
         check_verify(rows.to(dtype), tokens, [[-1, 0, 1]] * 6, mode="greedy")
 
 
+@pytest.mark.parametrize("V", [1, 2, 3, 4, 7, 8, 9, 15, 17, 511, 513, 1025, 8191, 8200, 33000])
+def test_greedy_finds_every_place(V):
+    # the largest at chosen places, on a floor of -inf, of equal values, and NaN of either sign
+    places = sorted({0, 1, 3, 7, 8, V // 2, V - 9, V - 8, V - 2, V - 1} & set(range(V)))
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        rows = torch.full((4 * len(places), 2, V), float("-inf"))
+        for k, at in enumerate(places):
+            rows[4 * k, :, at] = -3.0
+            rows[4 * k + 1] = -1.0
+            rows[4 * k + 1, :, at:] = 1.5
+            rows[4 * k + 2] = float("inf")
+            rows[4 * k + 2, :, at] = float("nan")
+            rows[4 * k + 3] = -0.0
+            rows[4 * k + 3, :, :at] = -5.0
+            rows[4 * k + 3, :, V - 1] = 0.0
+        logits = rows.to(dtype)
+        logits[2::4] = logits[2::4] * -1 if V % 2 else logits[2::4]  # (-inf around it, and NaN's sign turned)
+        check_verify(logits, [[0, at] for at in places for _ in range(4)], [[-1, 0]] * len(rows))
+
+
+@pytest.mark.parametrize("B,N,V,dtype", [(2, 300, 60001, torch.float16), (3, 20, 300000, torch.float32),
+                                         (2, 300, 50001, torch.bfloat16)])
+def test_greedy_of_many_rows(B, N, V, dtype):
+    # the first two read their rows on the walk (over 64 MiB of logits), the last one reads all of them first
+    r = random.Random(V)
+    logits = torch.randn((B, N, V), generator=torch.Generator(DEV).manual_seed(V), device=DEV).to(dtype).cpu()
+    parents = [random_tree(r, N, N) for _ in range(B)]
+    best = [[int((row == row.max()).nonzero()[0]) for row in seq] for seq in logits]
+    tokens = [[0] + [best[b][max(parents[b][i], 0)] if r.random() < 0.7 else r.randrange(V) for i in range(1, N)]
+              for b in range(B)]
+    got = check_verify(logits, tokens, parents)
+    assert max(got.counts.tolist()) > 2
+
+
+@pytest.mark.parametrize("mode", ["picks", "iid", "tree"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_verify_parts_of_the_vocabulary(mode, dtype):
+    # parts of more than one block, a last one that is full, that is short, that is one token
+    for V in (4096, 4097, 65536, 135168, 270001):
+        target, tokens, parents, u, draft = make(3, 6, V, dtype, mode, seed=V, sharp=1.0)
+        for u0 in (0.001, 0.5, 0.9999):
+            check_verify(target, tokens, parents, [[u0] + [0.99] * 3 + row[4:] for row in u], draft, mode)
+
+
 def test_sampling_is_the_targets():
     """The first emitted token over many draws is distributed as the target's
     at node 0, whatever the draft: within five standard deviations of every
