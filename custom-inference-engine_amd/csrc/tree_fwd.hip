@@ -15,10 +15,12 @@
 // go to workgroups of their own.
 //
 // Keys. A piece, one workgroup's work, is a run of 32-token tiles of ONE
-// sequence. Every workgroup finds its own from the context lengths: with C the
-// tiles per piece that spreads all sequences' tiles over the launch's
-// workgroups, sequence b has ceil(tiles_b / C) pieces of nearly equal length,
-// so ragged batches balance and the host needs no lengths. A sequence of more
+// sequence. Every workgroup finds its own from the context lengths: with C tiles
+// per piece, sequence b has ceil(tiles_b / C) pieces of nearly equal length, so
+// ragged batches balance and the host needs no lengths. The launch has workgroups
+// for B + extra pieces, enough for C = ceil(all tiles / extra) whatever the lengths.
+// (The smallest C that they are enough for, found by bisection, takes a tenth off
+// the longest piece and nothing off the time: the whole chip's rate bounds it.) A sequence of more
 // pieces than one leaves partial states (acc, m, l) that tree_merge_kernel
 // combines in a fixed order.
 //
@@ -51,6 +53,7 @@ struct TreeCfg {
   static constexpr int DT = D >= 32 ? D / 32 : 1;  // 32-column output tiles
   static constexpr int S = D / 8;                  // 16-byte chunks per head row
   static constexpr int QTI = QT < D / 16 ? QT : D / 16;  // waves of a head that issue its copies
+  static constexpr bool PAIR = QT == 8;            // two waves a SIMD, half a step apart
   static constexpr int CPW = D / (16 * QTI);             // 1 KiB copies per issuing wave, tensor and tile
 };
 
@@ -203,26 +206,27 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   const int tlo = (j - j0) * per_piece, thi = min(t, tlo + per_piece), T = thi - tlo;
   const int base = ctx - p.N;
 
-  // ---- block ids of the piece ------------------------------------------------
+  // ---- block ids of the piece, query fragments ----------------------------------
+  // What depends on the piece alone is asked for at once: block ids, q, depth. The
+  // rotation's table entries follow, then the first copies; q is rotated behind them
+  // (waiting for each in turn, the start took two more round trips to memory).
   const int blk_lo = (int)fdiv((uint32_t)(kPagedTile * tlo), p.bsdiv);
   const int nids = (int)fdiv((uint32_t)(min(ctx, kPagedTile * thi) - 1), p.bsdiv) - blk_lo + 1;
-  {
-    const int32_t* src = p.bt + (int64_t)b * p.max_blocks + blk_lo;
-    for (int x = threadIdx.x; x < nids; x += blockDim.x) {
-      const int id = src[x];
-      sbt[x] = (uint32_t)id < (uint32_t)p.num_blocks ? id : -1;
-    }
-  }
-
+  const int32_t* const src = p.bt + (int64_t)b * p.max_blocks + blk_lo;
+  const int id0 = src[min((int)threadIdx.x, nids - 1)];
   u32x4 qf[C::KK];
   const uint16_t* const qrow = p.q + (int64_t)b * p.qs0 + hq * p.qs1 + (int64_t)node * p.qs2;
 #pragma unroll
   for (int kk = 0; kk < C::KK; ++kk) qf[kk] = load16(qrow + 16 * kk + 8 * hl, rv);
-  if (p.rope.cos)  // node i is rotated at position base + its depth
-    rope_q_lane<DTYPE, D>(qf, p.rope, base + max(p.depths[(int64_t)b * p.ds0 + node], 0), rv, hl);
-#pragma unroll
-  for (int kk = 0; kk < C::KK; ++kk) qf[kk] ^= u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
+  const int depth = p.rope.cos ? p.depths[(int64_t)b * p.ds0 + node] : 0;
+  if ((int)threadIdx.x < nids) sbt[threadIdx.x] = (uint32_t)id0 < (uint32_t)p.num_blocks ? id0 : -1;
+  for (int x = threadIdx.x + blockDim.x; x < nids; x += blockDim.x) {
+    const int id = src[x];
+    sbt[x] = (uint32_t)id < (uint32_t)p.num_blocks ? id : -1;
+  }
   for (int x = threadIdx.x; x < p.HG * kTreeOddWords; x += blockDim.x) odd[x] = 0;
+  RopeRow<D> rr;
+  if (p.rope.cos) rr = rope_row_load<D>(p.rope, base + max(depth, 0), hl);  // node i at base + its depth
   __syncthreads();
   bool bad = false;
   for (int x = lane; x < nids; x += 64) bad |= sbt[x] < 0;
@@ -284,9 +288,12 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
                   st + 2u * TILE_EL + 1024u * x);
     }
   };
-  const int reach = NST - 1;  // step k copies tile k + reach
+  const int reach = NST - (C::PAIR ? 2 : 1);  // step k copies tile k + reach
   if (issuer)
     for (int k = 0; k < min(reach, T); ++k) issue(k);
+  if (p.rope.cos) rope_row_apply<DTYPE, D>(qf, p.rope, rr, rv, hl);
+#pragma unroll
+  for (int kk = 0; kk < C::KK; ++kk) qf[kk] ^= u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
 
   // ---- tile loop -------------------------------------------------------------
   // Byte addresses inside a tile. K row l32, chunk hh S + 2 kk + hl: the kk part is
@@ -342,10 +349,13 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   //
   // One barrier a step, between the two parts: behind it every wave has read V of tile
   // k - 1 (whose stage the softmax part refills) and every wave's copies of tile k + 1
-  // are done. (Eight waves in two halves, one in its matrix part while the other is in
-  // its softmax, kept apart by a barrier after each part: 88 -> 90 us for four trees of
-  // 64 nodes over 8192-16384 tokens, 42 -> 51 for 32 of 16 over 256-4096; the halves
-  // wait for one another more than they overlap.)
+  // are done. With two waves on a SIMD (QT = 8) the second one takes its matrix part
+  // behind the barrier, so that it multiplies while the first one is in its softmax;
+  // the ring then refills a stage one step later. The matrix part runs at a raised
+  // wave priority: the products are issued first, the other wave's softmax in between.
+  // Four trees of 64 nodes over 8192-16384 tokens: 86 us in step, 84.5 half a step
+  // apart, 81.5 with the priority. (Two halves kept apart by a barrier after each part:
+  // 90; they wait for one another more than they overlap.)
   u32x4 vf[2 * C::DT], kf[C::KK];
   auto load_key = [&](int st, int kk) __attribute__((always_inline)) {
     kf[kk] = lds_read16_at((ring_lds + 2u * (uint32_t)(st * STAGE_EL) + k_lane) ^ (32u * kk));
@@ -362,27 +372,34 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   for (int kk = 0; kk < C::KK; ++kk) load_key(0, kk);
   if (whole == 0) tidy(0, 0);
   int st_cur = 0, st_prev = 0;  // stages of tiles k and k - 1
-  for (int k = 0; k <= T; ++k) {
+  auto values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int dt = 0; dt < C::DT; ++dt) acc[dt] = E::mfma(vf[2 * dt + cc], pb[cc], acc[dt]);
+  };
+  auto matrix = [&](int k) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
     sc = f32x16{};
 #pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) {  // (k = T: a product of no use)
+    for (int kk = 0; kk < C::KK; ++kk) {
       sc = E::mfma(kf[kk], qf[kk], sc);
       if (kk < 2 * C::DT) load_value(st_prev, kk);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (D < 32) load_value(st_prev, 1);
-    if (k > 0) {
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-        for (int dt = 0; dt < C::DT; ++dt) acc[dt] = E::mfma(vf[2 * dt + cc], pb[cc], acc[dt]);
-      if (k == T) break;
-    }
+    if (k > 0) values();
+    __builtin_amdgcn_s_setprio(0);
+  };
+  const bool late = C::PAIR && w >= 4;
+  for (int k = 0; k < T; ++k) {
+    if (!late) matrix(k);
     const int st_next = st_cur + 1 == NST ? 0 : st_cur + 1;
     if (issuer && k + 1 < T) tree_wait<2 * C::CPW>(min(reach - 2, T - 2 - k));
     __syncthreads();
     if (issuer && k + reach < T) issue(k + reach);
     if (k + 1 >= whole && k + 1 < T) tidy(k + 1, st_next);
+    if (late) matrix(k);
     if (k >= whole) {  // the tile reaches past the history: the row's mask decides
       const uint32_t vis = tree_bits(words, kPagedTile * (tlo + k) - base, p.N, p.W, live) >> (4 * hl);
 #pragma unroll
@@ -414,6 +431,9 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
     st_prev = st_cur;
     st_cur = st_next;
   }
+#pragma unroll
+  for (int f = 0; f < 2 * C::DT; ++f) load_value(st_prev, f);
+  values();
 
   // ---- values that are not finite ----------------------------------------------
   if (whole < T) {
@@ -501,7 +521,10 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
   const uint32_t x = blockIdx.x * 256u + threadIdx.x;
   const uint32_t row = fdiv(x, p.updiv);  // node
   if (row >= (uint32_t)p.N) return;
+  // (everything that depends on the arguments alone is asked for before anything is
+  // waited for; block id and table entries, which depend on the length, together)
   const int ctx = p.lens[b];
+  const int depth = p.rope.cos ? p.depths[(int64_t)b * p.ds0 + row] : 0;
   const uint32_t c = x - row * p.updiv.d;
   const int half = p.D / 2, h = (int)(c / (uint32_t)(p.D / 16)), d = 8 * (int)(c % (uint32_t)(p.D / 16));
   const int64_t r = (int64_t)b * p.N + row;
@@ -509,16 +532,17 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
   const uint16_t* vs = p.vn + r * p.vns0 + h * p.vns1 + d;
   u32x4 k0 = *reinterpret_cast<const u32x4*>(ks), k1 = *reinterpret_cast<const u32x4*>(ks + half);
   const u32x4 v0 = *reinterpret_cast<const u32x4*>(vs), v1 = *reinterpret_cast<const u32x4*>(vs + half);
-  if (!tree_ctx_valid(p, ctx) || !tree_row_live(p.mask + (int64_t)b * p.ms0 + (int64_t)row * p.ms1, p.N)) return;
+  const bool live = tree_row_live(p.mask + (int64_t)b * p.ms0 + (int64_t)row * p.ms1, p.N);
+  if (!tree_ctx_valid(p, ctx) || !live) return;
   const int pos = ctx - p.N + (int)row;
   const int blk = (int)fdiv((uint32_t)pos, p.bsdiv), off = pos - blk * p.block_size;
   const int id = p.bt[(int64_t)b * p.max_blocks + blk];
-  if ((uint32_t)id >= (uint32_t)p.num_blocks) return;
   if (p.rope.cos) {
-    const int at = ctx - p.N + max(p.depths[(int64_t)b * p.ds0 + row], 0);
+    const int at = ctx - p.N + max(depth, 0);
     if (at >= p.rope.rows) return;
     rope_apply8<DTYPE>(k0, k1, rope_load(p.rope, (int64_t)at * half + d), p.rope.dt);
   }
+  if ((uint32_t)id >= (uint32_t)p.num_blocks) return;
   uint16_t* kd = const_cast<uint16_t*>(p.kc) + (int64_t)id * p.ks0 + (int64_t)off * p.ks1 + (int64_t)h * p.ks2 + d;
   uint16_t* vd = const_cast<uint16_t*>(p.vc) + (int64_t)id * p.vs0 + (int64_t)off * p.vs1 + (int64_t)h * p.vs2 + d;
   *reinterpret_cast<u32x4*>(kd) = k0;
@@ -540,10 +564,14 @@ __global__ __launch_bounds__(64 * kTreeMergeWaves) void tree_merge_kernel(const 
   __shared__ float2 sm[kTreeMergeWaves][64];
   const int b = blockIdx.y;
   const int2 inf = p.info[b];
-  if (inf.y < 2) return;  // written whole by the main pass
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hl = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hl = lane >> 5;
   const int cg = blockIdx.x % (D / 8), rg = blockIdx.x / (D / 8);  // rg = kvh * G32 + row group
   const int kvh = rg / p.G32, r = (rg - kvh * p.G32) * 32 + l32;
+  const int g = (int)fdiv((uint32_t)r, p.ndiv), i = r - g * p.N;
+  // (asked for along with the piece count, not after the last partial state)
+  const bool live = w == 0 && r < p.R && tree_row_live(p.mask + (int64_t)b * p.ms0 + (int64_t)i * p.ms1, p.N);
+  if (inf.y < 2) return;  // written whole by the main pass
   float M = -INFINITY, L = 0.f;
   float4 A = {0.f, 0.f, 0.f, 0.f};
   if (r < p.R)
@@ -567,8 +595,6 @@ __global__ __launch_bounds__(64 * kTreeMergeWaves) void tree_merge_kernel(const 
   if (w != 0 || r >= p.R) return;
 #pragma unroll
   for (int x = 1; x < kTreeMergeWaves; ++x) merge_state(M, L, A, sm[x][lane].x, sm[x][lane].y, sa[x][lane]);
-  const int g = (int)fdiv((uint32_t)r, p.ndiv), i = r - g * p.N;
-  const bool live = tree_row_live(p.mask + (int64_t)b * p.ms0 + (int64_t)i * p.ms1, p.N);
   const float inv = 1.f / L;
   uint16_t* orow = p.o + (int64_t)b * p.os0 + (int64_t)(kvh * p.group + g) * p.os1 + (int64_t)i * p.os2;
   *reinterpret_cast<u32x2*>(orow + 8 * cg + 4 * hl) =
