@@ -1094,6 +1094,7 @@ int cie_draft_masks(const int32_t* parents, int32_t* mask, int32_t* depths, uint
     g_err.clear();
     return CIE_OK;
   }
+  if (B > cie::kTreeMaxBatch) return fail(CIE_EINVAL, "problem too large for one launch");
   if (!parents || !mask || !depths) return fail(CIE_EINVAL, "parents / mask / depths: NULL pointer");
   return launch_status(cie::launch_draft_masks(parents, mask, depths, status, B, N, static_cast<hipStream_t>(stream)));
 }
@@ -1113,6 +1114,7 @@ static int verify_impl(const void* target, const void* draft, const void* draft_
     g_err.clear();
     return CIE_OK;
   }
+  if (B > cie::kTreeMaxBatch) return fail(CIE_EINVAL, "problem too large for one launch");
   if (V < 1) return fail(CIE_EINVAL, "the vocabulary is empty");
   if (token_bytes != 4 && token_bytes != 8) return fail(CIE_EINVAL, "tokens of %d bytes, expected 4 or 8", token_bytes);
   if (!target || !draft_tokens || !parents || !tokens || !path || !counts || !ts)

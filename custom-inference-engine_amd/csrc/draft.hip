@@ -667,7 +667,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_greedy_kernel(const Ver
 // 64 x 26 (106 MB) 26.9 / 20.2.
 size_t verify_tops_bytes(int B, int N, int V, int dtype) {
   const int64_t rows = (int64_t)B * N;
-  if (rows > (64ll << 20) / ((int64_t)V * (dtype == 2 ? 4 : 2))) return 0;
+  if (rows > (64ll << 20) / ((int64_t)V * (dtype == 2 ? 4 : 2)) || rows > 1 << 20) return 0;  // (and one launch)
   return (size_t)rows * kTopParts * sizeof(uint64_t);
 }
 

@@ -224,6 +224,7 @@ int build_paged_plan(int32_t* P, const PagedGeom& g, const PlanLayout& L, const 
 // Attention of a tree of N drafted tokens over the paged pool (tree_fwd.hip).
 constexpr int kTreeIds = 1024;       // block ids of a piece staged in LDS
 constexpr int kTreeMaxNodes = 1024;  // nodes of one tree
+constexpr int kTreeMaxBatch = (1 << 22) - 1;  // trees of a launch with a workgroup of up to 1024 threads for each
 constexpr int kTreeOddWords = kTreeMaxNodes / 32 + 2;  // tiles that reach past the history
 // Most threads of a workgroup with QT waves to a kv head: heads of at most 256
 // elements in all, eight waves (two to a SIMD; at D = 256 a wave needs a SIMD's

@@ -663,7 +663,9 @@ TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int b
   const int64_t units = pieces * g.NG;
   const int64_t nx = (int64_t)1 << dev.xcd_shift;
   const int64_t wgs = g.NRT > 1 ? (units + nx - 1) / nx * nx * g.NRT : units;
-  if (wgs > INT_MAX || B > 65535 || (int64_t)Hk * g.G32 * (D / 8) > INT_MAX) {
+  // (a grid dimension holds less than 2^32 threads)
+  if (wgs * (64 * g.HG * g.QT) > UINT_MAX || B > 65535 ||
+      (int64_t)Hk * g.G32 * (D / 8) * (64 * kTreeMergeWaves) > UINT_MAX) {
     g.err = "problem too large for one launch";
     return g;
   }

@@ -223,7 +223,8 @@ def kv_keep(k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor], 
     to ``starts[b] + j`` for j < ``counts[b]``.
 
     k_caches / v_caches: the layers' pools, all of one shape, 16-bit type and
-    layout. block_tables (B, max_blocks), starts (B,), counts (B,): int32 or
+    layout, each given once; a block that a moved row comes from or goes to
+    belongs to one sequence. block_tables (B, max_blocks), starts (B,), counts (B,): int32 or
     int64 on the device; path (B, N), ``Verified.path``: rising, entry j at
     least j. An entry outside [j, N) and a position whose block is out of range
     move nothing."""
@@ -545,7 +546,10 @@ class PagedKVCache:
     def keep_step(self, step: "StepBatch", path: torch.Tensor, counts: torch.Tensor) -> None:
         """The accepted paths of a step of draft trees (``Verified.path`` and
         ``.counts`` on the device): :func:`kv_keep` over every layer. No host
-        work; :meth:`rollback_step` follows when the counts are known."""
+        work; :meth:`rollback_step` follows when the counts are known. The step
+        is the trees' own: N new tokens at the end of every sequence."""
+        if path.dim() != 2 or len(path) and (step.num_new != path.shape[1] or not step.aligned):
+            raise ValueError(f"keep_step: paths of shape {tuple(path.shape)} and a step of {step.num_new} new tokens")
         kv_keep(self.k, self.v, step.block_tables, step.starts, path, counts)
 
     def rollback_step(self, step: "StepBatch", counts: Sequence[int]) -> None:

@@ -189,7 +189,7 @@ def accept_draft(cache, step, parents: torch.Tensor, draft_tokens: torch.Tensor,
     """The end of a tree step (``step = cache.prepare_step(tables, N)``, all
     layers run): verifies the drafts, greedily by logits when ``uniforms`` is
     None, and moves the accepted paths' K and V behind the histories in every
-    layer (``PagedKVCache.keep_step``). Two launches, nothing waits; once the
+    layer (``PagedKVCache.keep_step``). Two or three launches, nothing waits; once the
     program has read the counts, ``cache.rollback_step(step, counts)`` shortens
     the sequences to what they keep."""
     if uniforms is None:

@@ -588,7 +588,9 @@ int cie_verify_greedy(const void* target_logits, const void* draft_tokens, int t
  * outside [0, num_blocks) moves nothing. k_caches, v_caches: `layers` device
  * pointers in HOST memory, read during the call. Strides in bytes {block,
  * token, head}, the same for every layer's K and every layer's V, multiples of
- * 16; a head row is head_bytes bytes. path_stride: ints between sequences.
+ * 16; a head row is head_bytes bytes. path_stride: ints between sequences. The
+ * pools are all different, and a block that a moved row comes from or goes to
+ * belongs to one sequence (otherwise two moves of a row race).
  * Reference: engine/cache/kv_cache.py:187-194 rolls back a rejected chain.
  */
 int cie_kv_keep(void* const* k_caches, void* const* v_caches, int layers, const int64_t* k_stride,
