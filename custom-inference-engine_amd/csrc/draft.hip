@@ -80,8 +80,8 @@ hipError_t launch_draft_masks(const int32_t* parents, int32_t* mask, int32_t* de
 // pass over the rows per rejection gives W (one per node for the draft's own
 // picks, whose W follows from the children's p), and none is needed before a
 // first rejection: each child's p(x), q(x) and u are fetched once for the whole
-// tree, one thread a node. A step down the tree costs 0.5 us then, the start and
-// the end 4 us, and the passes the rest.
+// tree, one thread a node, and with them whether the child passes if it is the
+// first one tried.
 //
 // All sums are 64-bit: the last token is a comparison of a sum over the
 // vocabulary with u_0 times that sum, and has to come out the same whatever the
@@ -155,12 +155,14 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// Children of node `cur` after node `after`: the next one, or -1 (every wave
-// finds it for itself).
-__device__ __forceinline__ int next_child(const int32_t* par, int N, int cur, int after, int lane) {
+// Children of node `cur` after node `after`: the next one (with token x, if `tok`
+// is given), or -1; every wave finds it for itself.
+__device__ __forceinline__ int next_child(const int32_t* par, int N, int cur, int after, int lane,
+                                          const int32_t* tok = nullptr, int x = 0) {
   for (int c = (after + 1) >> 6; 64 * c < N; ++c) {
     const int i = 64 * c + lane;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(i < N && i > after && par[i] == cur);
+    const uint64_t m =
+        __builtin_amdgcn_ballot_w64(i < N && i > after && par[i] == cur && (!tok || tok[i] == x));
     if (m) return 64 * c + __builtin_ctzll(m);
   }
   return -1;
@@ -311,10 +313,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
   __shared__ double kept[kTreeMaxNodes];  // drafts without replacement: what p has left of a token that q lost
   __shared__ double ug[kTreeMaxNodes];
   __shared__ double psum[2][kParts], pq[kParts], wpre[kVerifyWaves];
+  __shared__ int32_t first_of[kTreeMaxNodes];  // a node's first child
+  __shared__ uint8_t easy[kTreeMaxNodes];      // accepted if nothing was rejected before it
   __shared__ int found, lastpos;
   const int b = blockIdx.x, i = threadIdx.x, lane = i & 63;
   const int w = __builtin_amdgcn_readfirstlane(i >> 6);
   const int N = p.N, V = p.V;
+  if (i < N) first_of[i] = N;
+  __syncthreads();
   const T* const target = static_cast<const T*>(p.target) + (int64_t)b * p.ts0;
   const T* const draft = MODE == kDraftPicks ? nullptr : static_cast<const T*>(p.draft) + (int64_t)b * p.ds0;
   if (i < N) {
@@ -327,6 +333,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
     qg[i] = child && MODE != kDraftPicks ? E::at(draft + (int64_t)up * p.ds1 + x) : 1.f;
     ug[i] = p.uniform_bytes == 8 ? static_cast<const double*>(p.uniforms)[(int64_t)b * N + i]
                                  : (double)static_cast<const float*>(p.uniforms)[(int64_t)b * N + i];
+    const double r = MODE == kDraftPicks ? (double)pg[i] : __builtin_fmax((double)pg[i], 0.0);
+    easy[i] = child && ug[i] * (double)qg[i] < r;
+    if (child) atomicMin(&first_of[up], i);
   }
   if (i == 0) found = V, lastpos = -1;
   __syncthreads();
@@ -373,12 +382,18 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draft_kernel(const Veri
       return -1;
     };
     for (;;) {
+      if (first_of[cur] < N && easy[first_of[cur]]) {  // the common step: two reads of LDS
+        cur = first_of[cur];
+        if (i == 0) path[count] = cur;
+        ++count;
+        continue;
+      }
       P = target + (int64_t)cur * p.ts1;
       if (MODE != kDraftPicks) Q = draft + (int64_t)cur * p.ds1;
       W = 1.0, c = 0.0, S = 1.0, total = 0.0, nlist = 0, have = false;
       bool first = true;  // no rejection at this node yet
       int taken = -1;
-      for (int ch = next_child(par, N, cur, cur, lane); ch >= 0; ch = next_child(par, N, cur, ch, lane)) {
+      for (int ch = first_of[cur] < N ? first_of[cur] : -1; ch >= 0; ch = next_child(par, N, cur, ch, lane)) {
         const int x = tok[ch];
         int at = MODE == kDraftIid ? -1 : place(x);
         const bool out = at >= 0 && gone[at];  // out of p (picks) or of q (no replacement)
@@ -639,8 +654,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_greedy_kernel(const Ver
       buf ^= 1;  // (the next node's do not overwrite what another wave still reads)
       t = (int)~(uint32_t)top;
     }
-    int ch = next_child(par, N, cur, cur, lane);
-    while (ch >= 0 && tok[ch] != t) ch = next_child(par, N, cur, ch, lane);
+    const int ch = next_child(par, N, cur, cur, lane, tok, t);
     if (ch < 0) {
       last = t;
       break;

@@ -139,6 +139,7 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   extern __shared__ __attribute__((aligned(1024))) uint16_t ring[];
   int32_t* const sbt = reinterpret_cast<int32_t*>(ring + p.NST * (2 * kPagedTile * 8) * p.NCH);
   uint32_t* const odd = reinterpret_cast<uint32_t*>(sbt + kTreeIds);  // [HG][kTreeOddWords] keys whose V is not finite
+  uint32_t* const seen = odd + p.HG * kTreeOddWords;                  // [tile past the history][32 QT rows] mask bits
 
   // (piece j, head group gh) = unit u, row tile rt; the row tiles of a unit are
   // 2^xcd_shift workgroup ids apart, so that they share an XCD's L2
@@ -225,6 +226,13 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
     sbt[x] = (uint32_t)id < (uint32_t)p.num_blocks ? id : -1;
   }
   for (int x = threadIdx.x; x < p.HG * kTreeOddWords; x += blockDim.x) odd[x] = 0;
+  const int whole = min(max(base / kPagedTile - tlo, 0), T);  // tiles of history alone
+  // the mask bits of the other tiles, a row's once for all heads (read from memory in
+  // the loop, they waited there for every copy under way)
+  if (hh == 0 && hl == 0)
+#pragma unroll 4
+    for (int x = whole; x < T; ++x)
+      seen[(x - whole) * (32 * QT) + 32 * qt + l32] = tree_bits(words, kPagedTile * (tlo + x) - base, p.N, p.W, live);
   RopeRow<D> rr;
   if (p.rope.cos) rr = rope_row_load<D>(p.rope, base + max(depth, 0), hl);  // node i at base + its depth
   __syncthreads();
@@ -321,7 +329,6 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   for (int dt = 0; dt < C::DT; ++dt) acc[dt] = f32x16{};
   float mx = -INFINITY, l = 0.f;
   const float c = p.scale_log2;
-  const int whole = min(max(base / kPagedTile - tlo, 0), T);  // tiles of history alone
   f32x16 sc = f32x16{};        // scores of the tile, then its probabilities
   u32x4 pb[2] = {};            // those in 16 bits
 
@@ -401,7 +408,7 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
     if (k + 1 >= whole && k + 1 < T) tidy(k + 1, st_next);
     if (late) matrix(k);
     if (k >= whole) {  // the tile reaches past the history: the row's mask decides
-      const uint32_t vis = tree_bits(words, kPagedTile * (tlo + k) - base, p.N, p.W, live) >> (4 * hl);
+      const uint32_t vis = seen[(k - whole) * (32 * QT) + 32 * qt + l32] >> (4 * hl);
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = (vis >> (8 * (e >> 2) + (e & 3))) & 1u ? sc[e] : -INFINITY;
     }
@@ -455,7 +462,7 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
           for (int y = 0; y < 8; ++y) s = fmaf(kv[y], qv[y], s);
         }
         s = xhalf_sum(s) * c;
-        const bool seen = live && (a < 0 || (words[a >> 5] >> (a & 31)) & 1);
+        const bool sees = live && (a < 0 || (words[a >> 5] >> (a & 31)) & 1);
         const float pe = exp2_fast(s - (mx == -INFINITY ? 0.f : mx));
 #pragma unroll
         for (int dt = 0; dt < C::DT; ++dt)
@@ -467,7 +474,7 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
             for (int y = 0; y < 4; ++y) {
               const uint32_t h = y & 1 ? v4[y >> 1] >> 16 : v4[y >> 1] & 0xffffu;
               const float add = pe * widen<DTYPE>(h);
-              acc[dt][4 * g4 + y] += (seen & ((h & kExp<DTYPE>) == kExp<DTYPE>)) ? add : 0.f;
+              acc[dt][4 * g4 + y] += (sees & ((h & kExp<DTYPE>) == kExp<DTYPE>)) ? add : 0.f;
             }
           }
       }
@@ -633,25 +640,33 @@ TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int b
   g.NST = std::min(8, std::max(3, (int)((size_t)128 * 1024 / stage)));
   const int cpt = 2 * (D / (16 * std::min(g.QT, D / 16)));  // copies of an issuing wave per tile
   g.NST = std::min(g.NST, 3 + 63 / cpt);                    // those of NST - 3 tiles in flight fit vmcnt
-  g.lds_bytes = (size_t)g.NST * stage + sizeof(int32_t) * (kTreeIds + g.HG * kTreeOddWords);
+  // nor more stages than the longest sequence has tiles (and those that reach leaves
+  // free): short ones then share a CU
+  const int64_t most = (ctx_limit + kPagedTile - 1) / kPagedTile + (g.QT == 8 ? 2 : 1);
+  g.NST = (int)std::min<int64_t>(g.NST, std::max<int64_t>(most, 2));
+  // behind the ring: block ids, keys whose V is not finite, mask bits of the tiles past
+  // the history (34 KiB for 1024 nodes, two stages less)
+  const size_t behind = sizeof(int32_t) * (kTreeIds + g.HG * kTreeOddWords + (size_t)(N / 32 + 2) * 32 * g.QT);
+  while (g.NST > 3 && (size_t)g.NST * stage + behind > kPagedLdsBudget) --g.NST;
+  g.lds_bytes = (size_t)g.NST * stage + behind;
   const int64_t nt_max = (int64_t)B * ((ctx_limit + kPagedTile - 1) / kPagedTile);
   // tiles whose block ids the workgroup can stage
   const int64_t ccap = std::max<int64_t>(1, ((int64_t)(kTreeIds - 2) * block_size) / kPagedTile);
-  // Pieces beyond one per sequence: while the sequences' workgroups take at most half
-  // of the CUs, what fills them once, one workgroup per CU. Above, k per sequence,
-  // k the number whose last round of workgroups leaves the least idle (sequences
-  // longer than 1 / k of the average are cut too); a cut costs the partial states,
-  // taken as 4 % (48 sequences of one length, 32/8 heads, D = 128: k = 2).
+  // Pieces beyond one per sequence. While the sequences' workgroups take at most half
+  // of the CUs: what fills them once, one workgroup per CU, in pieces of two tiles at
+  // least (one tile: 1 x 8 nodes over 777 tokens 12.0 -> 12.3 us; four: 13.5). Above
+  // that a piece has to pay for its start, the time of some six tiles, and for its
+  // partial states: only sequences of more than the average are cut, and of more than
+  // 32 tiles while every workgroup has a CU (10 of 11 nodes over 132-2112 tokens 50 us,
+  // of more than 64 tiles 68, than 8 51; 20 of 64 over 700-800 39.6, 39.0, 54.0), 64
+  // when they come in rounds (48 of 26 over 1000-2000 58, than 32 70). Against two to
+  // four pieces of two tiles or more per sequence: 41 of 110 over 33 tokens 68 -> 30,
+  // 22 of 64 over 900 87 -> 42, 17 of 200 over 300-4000 378 -> 256, 48 of 8 over 4000
+  // 158 -> 133; but 33 of 16 over 500-8000 108 -> 119, 48 of 26 over 2000-4000 126 -> 134.
   const int64_t per_piece = (int64_t)g.NG * g.NRT;
-  int64_t extra = std::max<int64_t>(1, dev.cus / per_piece - B);
-  if (2 * B * per_piece > dev.cus) {
-    double least = 0;
-    for (int k = 1; k <= 4; ++k) {
-      const double rounds = (double)((k * B * per_piece + dev.cus - 1) / dev.cus) / k + 0.04 * (k - 1);
-      if (k == 1 || rounds < least) least = rounds, extra = k * B;
-    }
-  }
-  g.cmin = (int)std::min<int64_t>(ccap, 2);  // (one tile: 1 x 8 nodes over 777 tokens 12.0 -> 12.3 us; four: 13.5)
+  const bool busy = 2 * B * per_piece > dev.cus;
+  int64_t extra = busy ? B : std::max<int64_t>(1, dev.cus / per_piece - B);
+  g.cmin = (int)std::min<int64_t>(ccap, !busy ? 2 : B * per_piece > dev.cus ? 64 : 32);
   extra = std::min(extra, std::max<int64_t>(1, (nt_max + g.cmin - 1) / g.cmin));
   extra = std::max(extra, (nt_max + ccap - 1) / ccap);
   if (extra > INT_MAX / 2) {

@@ -130,6 +130,30 @@ def test_many_sequences():
     c.check(c.run())
 
 
+@pytest.mark.parametrize("N,Hq,Hk,D", [(3, 2, 2, 64), (33, 2, 1, 128), (65, 4, 1, 32)])
+def test_many_sequences_some_of_them_cut(N, Hq, Hk, D):
+    # more workgroups than half of the CUs: only the longest sequences are split
+    r = random.Random(N)
+    c = Case([r.randint(0, 200) for _ in range(170)] + [5000, 2100 - N, 2048 - N, 2049 - N, 0], N, D, torch.bfloat16,
+             Hq=Hq, Hk=Hk, seed=N)
+    c.check(c.run(max_context=max(c.lens)), sequences=[0, 1, 50, 169, 170, 171, 172, 173, 174])
+    c.check(c.run(), sequences=[2, 100, 170, 172])
+
+
+@pytest.mark.parametrize("N,bases", [(1, [0] * 40), (5, [0, 27, 20] * 20), (33, [0, 31, 30, 62] * 12),
+                                     (100, [0, 28, 60] * 10), (200, [0, 24, 56])])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_short_sequences_share_a_cu(N, bases, D):
+    # one to eight tiles with a tight max_context: few stages in the ring
+    c = Case(bases, N, D, torch.float16, Hq=8, Hk=2 if N < 100 else 1, seed=N)
+    c.check(c.run(max_context=max(c.lens)), sequences=range(min(4, len(bases))))
+
+
+def test_largest_tree_over_a_history():
+    c = Case([777], 1024, 128, torch.float16, Hq=2, Hk=1, seed=2)
+    c.check(c.run())
+
+
 @pytest.mark.parametrize("base", [0, 40, 3000])
 def test_padding_rows_are_zero(base):
     # trees of fewer nodes than slots, one sequence without any; a single long one splits over workgroups
