@@ -20,15 +20,23 @@
 // ragged batches balance and the host needs no lengths. The launch has workgroups
 // for B + extra pieces, enough for C = ceil(all tiles / extra) whatever the lengths.
 // (The smallest C that they are enough for, found by bisection, takes a tenth off
-// the longest piece and nothing off the time: the whole chip's rate bounds it.) A sequence of more
-// pieces than one leaves partial states (acc, m, l) that tree_merge_kernel
-// combines in a fixed order.
+// the longest piece and nothing off the time: the whole chip's rate bounds it.) A
+// sequence of more pieces than one leaves partial states (acc, m, l) that
+// tree_merge_kernel combines in a fixed order.
 //
 // Per tile: K and V go global -> LDS by 16-byte direct copies into a ring of NST
 // stages,
 //   S^T = K Q^T, online softmax in registers, O^T += V^T P^T
 // as in paged_fwd.hip. Only tiles that reach past the history look at the tree
-// mask: a lane cuts the 32 bits of the tile out of its row's words.
+// mask: the 32 bits of every row and tile are cut out of its words before the loop.
+//
+// Bounds. Few rows per kv head: the K / V bytes (32 trees of 16 nodes over 256-4096
+// tokens, 32/8 heads, D = 64: 141 MB, main pass 34-37 us, 4 TB/s). Many rows: products
+// and softmax at the clock that the board's power leaves (four trees of 64 nodes over
+// 8192-16384 tokens, 32/8 heads, D = 128: 55 GFLOP, main pass 72-80 us, of which the
+// tile loop 65 at 0.85 PFLOP/s, the first tile arriving after 6.5 and the partial
+// states, 33 MB, the rest). Short ones: the start, four dependent reads (lengths, block
+// ids, first tile, then the partial states of the merge).
 //
 // P is rounded to the 16-bit type for the second product, as in the dense and
 // paged kernels; its sum is fp32 and of the unrounded values.
@@ -519,7 +527,8 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
 // Writes the nodes' K and V behind the history before attention reads them:
 // node i of sequence b (rows b * N + i of kn / vn) to position base + i, K
 // rotated at base + its depth. One thread moves a pair of 16-byte chunks (the
-// two halves that a rotation mixes) of K and of V. Padding slots, positions
+// two halves that a rotation mixes) of K and of V. Bound by latency: 2.4 us for 1 x 8
+// nodes of 8 x 64, 3.4-4.9 for 8 x 26 of 8 x 128. Padding slots, positions
 // outside the rotary tables and invalid sequences are left as they are.
 template <int DTYPE>
 __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
@@ -561,7 +570,9 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
 // Combines the pieces of every sequence that has more than one: a workgroup
 // takes one column group (8 columns of 32 rows, 64 lanes x 4 values) and its
 // four waves the pieces in turn, each reading whole 1 KiB runs of the partial
-// states; the four results are joined in wave order.
+// states; the four results are joined in wave order. A launch and two dependent
+// reads (2.6-4 us), then the bytes: 33 MB in 9.2-10 us. (One wave a group, a quarter
+// of the workgroups: 10.0 -> 9.8 us there, 4.0 -> 4.7 at 13 pieces of 8 rows.)
 constexpr int kTreeMergeWaves = 4, kTreeMergeBatch = 4;
 
 template <int DTYPE, int D>
