@@ -310,6 +310,48 @@ def test_verify_in_a_graph_and_on_a_side_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_greedy_in_two_graphs_and_on_two_streams():
+    # each call has its own workspace: graphs replayed in turn and calls on two streams at once do not meet in it
+    r = random.Random(2)
+    trees = [[random_tree(r, 30, 30) for _ in range(3)] for _ in range(2)]
+    logits = [torch.randn((3, 30, 5000), device=DEV) for _ in range(2)]
+    tokens = [torch.zeros((3, 30), dtype=torch.int64, device=DEV) for _ in range(2)]
+    p = [dev(t) for t in trees]
+    up = [x.clamp(min=0).long() for x in p]
+
+    def refill(seed):
+        g = torch.Generator(DEV).manual_seed(seed)
+        for i in range(2):
+            logits[i].normal_(generator=g)
+            tokens[i].copy_(logits[i].argmax(-1).gather(1, up[i]))  # every child right: whole chains pass
+
+    refill(0)
+    verify_greedy(logits[0], tokens[0], p[0])
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            got.append(verify_greedy(logits[i], tokens[i], p[i]))
+    for seed in range(1, 4):
+        refill(seed)
+        want = [verify_greedy(logits[i], tokens[i], p[i]) for i in range(2)]
+        torch.cuda.synchronize()
+        for i in (0, 1, 0, 1):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        side = [torch.cuda.Stream() for _ in range(2)]
+        both = []
+        for i in range(2):
+            with torch.cuda.stream(side[i]):
+                both.append([verify_greedy(logits[i], tokens[i], p[i]) for _ in range(5)])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert max(want[i].counts.tolist()) > 3
+            for other in [got[i], *both[i]]:
+                assert all(torch.equal(a, b) for a, b in zip(want[i], other))
+
+
 def test_verify_refusals_and_empty():
     target, tokens, parents, u, draft = make(2, 5, 30, torch.float32, "tree", seed=1)
     t, d, x, p, uu = target.to(DEV), draft.to(DEV), dev(tokens, torch.int64), dev(parents), dev(u, torch.float32)

@@ -149,6 +149,13 @@ def test_short_sequences_share_a_cu(N, bases, D):
     c.check(c.run(max_context=max(c.lens)), sequences=range(min(4, len(bases))))
 
 
+def test_lengths_over_max_context_are_nan():
+    c = Case([10, 300, 40], 6, 64, torch.float16, seed=3)
+    out = c.run(max_context=64)
+    assert torch.isnan(out[1]).all()
+    c.check(out, sequences=[0, 2])
+
+
 def test_largest_tree_over_a_history():
     c = Case([777], 1024, 128, torch.float16, Hq=2, Hk=1, seed=2)
     c.check(c.run())
