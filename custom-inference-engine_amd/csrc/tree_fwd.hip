@@ -571,7 +571,7 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
 // takes one column group (8 columns of 32 rows, 64 lanes x 4 values) and its
 // four waves the pieces in turn, each reading whole 1 KiB runs of the partial
 // states; the four results are joined in wave order. A launch and two dependent
-// reads (2.6-4 us), then the bytes: 33 MB in 9.2-10 us. (One wave a group, a quarter
+// reads (2.4-3.7 us), then the bytes: 33 MB in 9.2-9.7 us. (One wave a group, a quarter
 // of the workgroups: 10.0 -> 9.8 us there, 4.0 -> 4.7 at 13 pieces of 8 rows.)
 constexpr int kTreeMergeWaves = 4, kTreeMergeBatch = 4;
 
@@ -597,12 +597,12 @@ __global__ __launch_bounds__(64 * kTreeMergeWaves) void tree_merge_kernel(const 
       float2 ml[kTreeMergeBatch];
       float4 a[kTreeMergeBatch];
 #pragma unroll
-      for (int u = 0; u < kTreeMergeBatch; ++u) {
-        const int k = min(k0 + kTreeMergeWaves * u, inf.y - 1);
-        const int64_t slot = (int64_t)(inf.x + k) * p.Hk * p.G32 + rg;
-        ml[u] = p.ml[slot * 32 + l32];
-        a[u] = *reinterpret_cast<const float4*>(p.part + slot * (32 * D) + 256 * cg + 4 * lane);
-      }
+      for (int u = 0; u < kTreeMergeBatch; ++u)
+        if (k0 + kTreeMergeWaves * u < inf.y) {
+          const int64_t slot = (int64_t)(inf.x + k0 + kTreeMergeWaves * u) * p.Hk * p.G32 + rg;
+          ml[u] = p.ml[slot * 32 + l32];
+          a[u] = *reinterpret_cast<const float4*>(p.part + slot * (32 * D) + 256 * cg + 4 * lane);
+        }
 #pragma unroll
       for (int u = 0; u < kTreeMergeBatch; ++u)
         if (k0 + kTreeMergeWaves * u < inf.y) merge_state(M, L, A, ml[u].x, ml[u].y, a[u]);
