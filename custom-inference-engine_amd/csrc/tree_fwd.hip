@@ -116,6 +116,11 @@ __device__ __forceinline__ bool tree_row_live(const int32_t* words, int N) {
   return any != 0;
 }
 
+// Rotary position of a node; a sum past 31 bits is past every table.
+__device__ __forceinline__ int tree_position(int base, int depth) {
+  return (int)min((uint32_t)base + (uint32_t)max(depth, 0), 0x7fffffffu);
+}
+
 template <int PT>
 __device__ __forceinline__ void tree_wait(int ahead) {
   // vmcnt counts the PT copies of every tile issued after the one needed
@@ -242,7 +247,7 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
     for (int x = whole; x < T; ++x)
       seen[(x - whole) * (32 * QT) + 32 * qt + l32] = tree_bits(words, kPagedTile * (tlo + x) - base, p.N, p.W, live);
   RopeRow<D> rr;
-  if (p.rope.cos) rr = rope_row_load<D>(p.rope, base + max(depth, 0), hl);  // node i at base + its depth
+  if (p.rope.cos) rr = rope_row_load<D>(p.rope, tree_position(base, depth), hl);
   __syncthreads();
   bool bad = false;
   for (int x = lane; x < nids; x += 64) bad |= sbt[x] < 0;
@@ -554,7 +559,7 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
   const int blk = (int)fdiv((uint32_t)pos, p.bsdiv), off = pos - blk * p.block_size;
   const int id = p.bt[(int64_t)b * p.max_blocks + blk];
   if (p.rope.cos) {
-    const int at = ctx - p.N + max(depth, 0);
+    const int at = tree_position(ctx - p.N, depth);
     if (at >= p.rope.rows) return;
     rope_apply8<DTYPE>(k0, k1, rope_load(p.rope, (int64_t)at * half + d), p.rope.dt);
   }

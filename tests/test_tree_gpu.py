@@ -328,6 +328,26 @@ def test_positions_outside_the_tables():
     assert torch.equal(k.view(-1, 2, 64)[at[deep]], before.view(-1, 2, 64)[at[deep]])
 
 
+def test_depths_of_any_value():
+    # a depth below 0 counts as 0; one that takes the position past the tables, or past 31 bits, makes a NaN row
+    c = Case([20], 6, 64, torch.float16, seed=15)
+    c.parents = [[-1, 0, 1, 2, 0, 4]]
+    tree = c.tree()
+    cos, sin = (t.to(DEV) for t in build_rope_cache(22, 64))
+    q, k, v, bt, lens = c.device()
+    new = (torch.ones(6, 2, 64, dtype=q.dtype, device=DEV),) * 2
+    before = k.clone()
+    depths = torch.tensor([[-5, 1, 2 ** 31 - 1, 2 ** 31 - 21, -2 ** 31, 2]], dtype=torch.int32, device=DEV)
+    out = tree_attention(q, k, v, bt, lens, tree.mask, rope=(cos, sin), depths=depths, new_kv=new)
+    deep = torch.tensor([0, 0, 1, 1, 0, 1], dtype=torch.bool, device=DEV)
+    assert torch.isnan(out[0][:, deep].float()).all()
+    at = c.slots(0)[20:].to(DEV)
+    assert torch.equal(k.view(-1, 2, 64)[at[deep]], before.view(-1, 2, 64)[at[deep]])
+    same = tree_attention(q, before, v.clone(), bt, lens, tree.mask, rope=(cos, sin), new_kv=new,
+                          depths=torch.tensor([[0, 1, 30, 30, 0, 30]], dtype=torch.int32, device=DEV))
+    assert torch.equal(out.isnan(), same.isnan()) and torch.equal(out.nan_to_num(), same.nan_to_num())
+
+
 def test_append_leaves_other_rows_and_invalid_sequences():
     c = Case([10, 30], 5, 32, torch.float16, seed=14, nodes=[3, 5])
     q, k, v, bt, lens = c.device()
