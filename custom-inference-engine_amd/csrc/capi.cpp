@@ -974,7 +974,7 @@ extern "C" {
 
 size_t cie_tree_workspace_bytes(int B, int Hq, int Hk, int N, int D, int max_context, int block_size,
                                 int max_blocks_per_seq) {
-  if (block_size < 1 || max_blocks_per_seq < 0 || (int64_t)max_blocks_per_seq * block_size > 0x7fffffff || Hk < 1) return 0;
+  if (block_size < 1 || max_blocks_per_seq < 0 || (int64_t)max_blocks_per_seq * block_size > 0x7fffffc0 || Hk < 1) return 0;
   const cie::TreeGeom g =
       tree_geom(B, Hq, Hk, N, D, paged_ctx_limit(max_context, block_size, max_blocks_per_seq), block_size);
   return g.ok ? g.info_bytes + g.ml_bytes + g.part_bytes : 0;
@@ -994,8 +994,8 @@ int cie_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_c
   if (num_blocks < 0 || max_blocks_per_seq < 0)
     return fail(CIE_EINVAL, "negative pool geometry (num_blocks=%d, max_blocks_per_seq=%d)", num_blocks,
                 max_blocks_per_seq);
-  if ((int64_t)max_blocks_per_seq * block_size > 0x7fffffff)
-    return fail(CIE_EINVAL, "max_blocks_per_seq * block_size exceeds 2^31");
+  if ((int64_t)max_blocks_per_seq * block_size > 0x7fffffc0)  // (a length rounded up to tiles stays an int)
+    return fail(CIE_EINVAL, "max_blocks_per_seq * block_size exceeds 2^31 - 64");
   if (!std::isfinite(scale)) return fail(CIE_EINVAL, "scale must be finite");
   if ((int64_t)B * N == 0) {
     g_err.clear();

@@ -43,7 +43,7 @@ def _tree(**over):
 @pytest.mark.parametrize("over,code", [
     (dict(D=48), "CIE_EHEADDIM"), (dict(dtype=2), "CIE_EDTYPE"), (dict(Hq=7), "CIE_EINVAL"), (dict(B=-1), "CIE_EINVAL"),
     (dict(N=-1), "CIE_EINVAL"), (dict(N=1025), "CIE_EINVAL"), (dict(bs=0), "CIE_EINVAL"),
-    (dict(num_blocks=-1), "CIE_EINVAL"), (dict(width=-1), "CIE_EINVAL"), (dict(width=1 << 28, bs=16), "CIE_EINVAL"),
+    (dict(num_blocks=-1), "CIE_EINVAL"), (dict(width=-1), "CIE_EINVAL"), (dict(width=1 << 28, bs=16), "CIE_EINVAL"), (dict(width=(1 << 31) - 1, bs=1), "CIE_EINVAL"),
     (dict(scale=math.nan), "CIE_EINVAL"), (dict(scale=math.inf), "CIE_EINVAL"), (dict(q=None), "CIE_EINVAL"),
     (dict(q=FAKE + 2), "CIE_EINVAL"), (dict(o=None), "CIE_EINVAL"), (dict(kc=FAKE + 8), "CIE_EINVAL"),
     (dict(vc=None), "CIE_EINVAL"), (dict(bt=None), "CIE_EINVAL"), (dict(lens=None), "CIE_EINVAL"),
