@@ -576,7 +576,7 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const TreeParams p) {
 // takes one column group (8 columns of 32 rows, 64 lanes x 4 values) and its
 // four waves the pieces in turn, each reading whole 1 KiB runs of the partial
 // states; the four results are joined in wave order. A launch and two dependent
-// reads (2.4-3.7 us), then the bytes: 33 MB in 9.2-9.7 us. (One wave a group, a quarter
+// reads (2.4-3.3 us), then the bytes: 33 MB in 9.2-9.7 us. (One wave a group, a quarter
 // of the workgroups: 10.0 -> 9.8 us there, 4.0 -> 4.7 at 13 pieces of 8 rows.)
 constexpr int kTreeMergeWaves = 4, kTreeMergeBatch = 4;
 
