@@ -31,15 +31,21 @@
 // mask: the 32 bits of every row and tile are cut out of its words before the loop.
 //
 // Bounds. Few rows per kv head: the K / V bytes (32 trees of 16 nodes over 256-4096
-// tokens, 32/8 heads, D = 64: 141 MB, main pass 34-37 us, 4 TB/s). Many rows: products
-// and softmax at the clock that the board's power leaves (four trees of 64 nodes over
-// 8192-16384 tokens, 32/8 heads, D = 128: 55 GFLOP, main pass 72-80 us, of which the
-// tile loop 65 at 0.85 PFLOP/s, the first tile arriving after 6.5 and the partial
-// states, 33 MB, the rest). Short ones: the start, four dependent reads (lengths, block
-// ids, first tile, then the partial states of the merge).
+// tokens, 32/8 heads, D = 64: 141 MB, main pass 37-38 us, 3.8 TB/s). Many rows: products
+// and softmax, which overlap in part only (four trees of 64 nodes over 8192-16384 tokens,
+// 32/8 heads, D = 128: 55 GFLOP, half as much again with the second part of P; main pass
+// 91-100 us, the first tile arriving after 6.5, the partial states 33 MB). Short ones:
+// the start, four dependent reads (lengths, block ids, first tile, then the partial
+// states of the merge).
 //
-// P is rounded to the 16-bit type for the second product, as in the dense and
-// paged kernels; its sum is fp32 and of the unrounded values.
+// P keeps two 16-bit parts for the second product, the rounded p and what the
+// rounding left (Elt::rest2), with a product for each; its sum is fp32 and of the
+// unrounded values. The output is then within its own rounding of the fp32 formula.
+// Relative error against 64 bits, one part / two parts / the output's rounding alone:
+// 32 x 16 in fp16 2.90e-4 / 2.07e-4 / 2.07e-4, 4 x 64 in bf16 2.34e-3 / 1.66e-3 /
+// 1.66e-3; time of the two calls 39.4 / 42.1 and 81.7 / 99.0 us. A seen V that is not
+// finite leaves its column of the row not finite: an infinity may come out as NaN,
+// its products with the two parts being of either sign.
 //
 // A masked key must not reach a row even if its V holds infinities or NaN (the
 // slots of padding nodes are never written): in a tile past the history such
@@ -342,8 +348,8 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   for (int dt = 0; dt < C::DT; ++dt) acc[dt] = f32x16{};
   float mx = -INFINITY, l = 0.f;
   const float c = p.scale_log2;
-  f32x16 sc = f32x16{};        // scores of the tile, then its probabilities
-  u32x4 pb[2] = {};            // those in 16 bits
+  f32x16 sc = f32x16{}, sn;      // scores of the tile, then its probabilities; scores of the next one
+  u32x4 pb[2] = {}, pr[2] = {};  // the probabilities in 16 bits, and what that rounding left
 
   // V of a tile past the history, before any wave reads it: values that are not
   // finite become zeros in LDS and their keys are noted, this wave's share of the
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   // behind the barrier, so that it multiplies while the first one is in its softmax;
   // the ring then refills a stage one step later. The matrix part runs at a raised
   // wave priority: the products are issued first, the other wave's softmax in between.
-  // Four trees of 64 nodes over 8192-16384 tokens: 86 us in step, 84.5 half a step
+  // Four trees of 64 nodes over 8192-16384 tokens, with P in one part: 86 us in step, 84.5 half a step
   // apart, 81.5 with the priority. (Two halves kept apart by a barrier after each part:
   // 90; they wait for one another more than they overlap.)
   u32x4 vf[2 * C::DT], kf[C::KK];
@@ -397,18 +403,34 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
     for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
       for (int dt = 0; dt < C::DT; ++dt) acc[dt] = E::mfma(vf[2 * dt + cc], pb[cc], acc[dt]);
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int dt = 0; dt < C::DT; ++dt) acc[dt] = E::mfma(vf[2 * dt + cc], pr[cc], acc[dt]);
+  };
+  // What the rounding of probabilities 2 w2 and 2 w2 + 1 left. A wave that has its SIMD
+  // to itself takes it between the score products of the next tile, which do not need
+  // the vector unit; two that share one in the softmax part, where the other wave
+  // multiplies (48 trees of 8 nodes over 4000 tokens, 32/8 heads, D = 128, all in the
+  // softmax part 148 -> 142 us; 4 x 64, all between the products 99 -> 103).
+  auto rest = [&](int w2) __attribute__((always_inline)) {
+    pr[w2 >> 2][w2 & 3] = E::rest2(pb[w2 >> 2][w2 & 3], sc[2 * w2], sc[2 * w2 + 1]);
   };
   auto matrix = [&](int k) __attribute__((always_inline)) {
     __builtin_amdgcn_s_setprio(1);
-    sc = f32x16{};
+    sn = f32x16{};
 #pragma unroll
     for (int kk = 0; kk < C::KK; ++kk) {
-      sc = E::mfma(kf[kk], qf[kk], sc);
+      sn = E::mfma(kf[kk], qf[kk], sn);
       if (kk < 2 * C::DT) load_value(st_prev, kk);
+      if (!C::PAIR)
+#pragma unroll
+        for (int w2 = 8 * kk / C::KK; w2 < 8 * (kk + 1) / C::KK; ++w2) rest(w2);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (D < 32) load_value(st_prev, 1);
     if (k > 0) values();
+    sc = sn;
     __builtin_amdgcn_s_setprio(0);
   };
   const bool late = C::PAIR && w >= 4;
@@ -444,8 +466,11 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
 #pragma unroll
       for (int e = 4 * e4; e < 4 * e4 + 4; ++e) sc[e] = exp2_fast(fmaf(sc[e], c, neg_m));
       l += (sc[4 * e4] + sc[4 * e4 + 1]) + (sc[4 * e4 + 2] + sc[4 * e4 + 3]);
-      pb[e4 >> 1][2 * (e4 & 1)] = E::pack2(sc[4 * e4], sc[4 * e4 + 1]);
-      pb[e4 >> 1][2 * (e4 & 1) + 1] = E::pack2(sc[4 * e4 + 2], sc[4 * e4 + 3]);
+#pragma unroll
+      for (int w2 = 2 * e4; w2 < 2 * e4 + 2; ++w2) {
+        pb[w2 >> 2][w2 & 3] = E::pack2(sc[2 * w2], sc[2 * w2 + 1]);
+        if (C::PAIR) rest(w2);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     st_prev = st_cur;
@@ -453,6 +478,9 @@ __global__ __launch_bounds__(tree_threads(D, QT)) void tree_fwd_kernel(const Tre
   }
 #pragma unroll
   for (int f = 0; f < 2 * C::DT; ++f) load_value(st_prev, f);
+  if (!C::PAIR)
+#pragma unroll
+    for (int w2 = 0; w2 < 8; ++w2) rest(w2);
   values();
 
   // ---- values that are not finite ----------------------------------------------

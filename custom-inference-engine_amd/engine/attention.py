@@ -577,7 +577,9 @@ def tree_attention(
     (``engine.decode.draft_tree(parents).mask``): node i sees the history and
     the nodes a whose bit a is set in its row. A row without a set bit is a
     padding slot; its output is zero. Keys that a row does not see have no
-    influence on it, whatever the pool holds there. N is at most 1024. Returns
+    influence on it, whatever the pool holds there. The probabilities keep two
+    16-bit parts: the result is within the output's own rounding of fp32
+    attention. N is at most 1024. Returns
     (B, Hq, N, D) in q's dtype; rows of a sequence with an invalid length or
     block id are NaN.
 

@@ -517,7 +517,9 @@ int cie_draft_masks(const int32_t* parents, int32_t* mask, int32_t* depths, uint
  * out; mask_batch_stride words between sequences, 0 for one tree for all). A
  * row without a set bit is a padding slot: it sees nothing, its output is
  * zero. What the pool holds at a position that a row does not see has no
- * influence on the row, NaN and infinities included. A context length outside
+ * influence on the row, NaN and infinities included; a value there that a row
+ * sees and that is not finite leaves its column of the row not finite (the
+ * probabilities keep two 16-bit parts: infinity may become NaN). A context length outside
  * [N, limit] or a block id outside [0, num_blocks) is never dereferenced: the
  * sequence's rows are NaN.
  * rope_cos, rope_sin (NULL: none): q is un-rotated, node i is rotated at

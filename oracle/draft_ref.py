@@ -44,7 +44,7 @@ def mask_words(seen: list[set[int]]) -> torch.Tensor:
 
 
 def tree_attention_f64(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, see: torch.Tensor,
-                       scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+                       scale: float, parts: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
     """One sequence: q (Hq, N, D), k / v (L, Hk, D), see (N, L) bool. Returns
     the outputs (Hq, N, D) in 64 bits (zero rows where a row sees nothing,
     masked keys left out of every sum) and, elementwise, how far a kernel may
@@ -53,7 +53,9 @@ def tree_attention_f64(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, see: t
 
     half a step of the output, half a step (or half the smallest 16-bit
     magnitude) of every probability times |v|, and for the fp32 sums of D
-    products per score and L terms per row, 2^-24 per addition."""
+    products per score and L terms per row, 2^-24 per addition. ``parts`` = 2:
+    a kernel that also keeps what the rounding of a probability left, rounded
+    to q's type, as a second term; half a step of half a step is lost then."""
     h = torch.finfo(q.dtype).eps / 2
     tiny = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2
     Hq, N, D = q.shape
@@ -73,9 +75,9 @@ def tree_attention_f64(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, see: t
             out[hq, i] = p @ vv
             a = p @ vv.abs()
             reach = float((kk.abs() @ qq.abs()).max()) * abs(scale)  # sum of |products| behind a score
-            eps32 = 2.0 ** -24 * (2 * (D + 8) * reach + L + 64)
+            eps32 = 2.0 ** -24 * (2 * (D + 8) * reach + parts * L + 64)
             # probabilities are rounded relative to the running maximum, the largest being up to 1
-            bound[hq, i] = h * out[hq, i].abs() + h * a * (1 + h) + tiny * (1 + top * vv.abs().sum(0)) + eps32 * a
+            bound[hq, i] = h * out[hq, i].abs() + h ** parts * a * (1 + h) + tiny * (1 + top * vv.abs().sum(0)) + eps32 * a
     return out, bound
 
 
