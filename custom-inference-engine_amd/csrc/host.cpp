@@ -700,8 +700,9 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (replacement < 0) return nullptr;
   const c10::OptionalDeviceGuard guard(t->device());
   const Tensor xc = x->contiguous(), pc = index32(*p), uc = u ? u->contiguous() : Tensor();
-  const Tensor tokens = at::empty({B, N}, xc.options()), path = at::empty({B, N}, pc.options()),
-               counts = at::empty({B}, pc.options());
+  const Tensor tokens = at::empty({B, N}, xc.options()), path = at::empty({B, N}, pc.options());
+  // (the library writes nothing for trees without nodes)
+  const Tensor counts = N ? at::empty({B}, pc.options()) : at::zeros({B}, pc.options());
   const Strides st(*t), sd(d ? *d : *t);
   const int tb = (int)xc.element_size();
   int32_t *const pp = static_cast<int32_t*>(path.data_ptr()), *const cp = static_cast<int32_t*>(counts.data_ptr());

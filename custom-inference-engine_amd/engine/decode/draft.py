@@ -46,7 +46,7 @@ class Verified(NamedTuple):
     """``tokens`` (B, N), like the drafted ones: the accepted nodes' tokens and
     the last one, then -1; ``path`` int32 (B, N): node 0 and the accepted nodes,
     then -1; ``counts`` int32 (B,): how many entries of both (0 for a sequence
-    whose node 0 is a padding slot)."""
+    whose node 0 is a padding slot, and for trees without nodes)."""
     tokens: torch.Tensor
     path: torch.Tensor
     counts: torch.Tensor
@@ -123,7 +123,8 @@ def _verify(name: str, target: torch.Tensor, draft_tokens: torch.Tensor, parents
     parents = parents.to(torch.int32).expand(B, N).contiguous()
     tokens = torch.empty_like(draft_tokens)
     path = torch.empty_like(parents)
-    counts = torch.empty((B,), dtype=torch.int32, device=target.device)
+    # (the library writes nothing for trees without nodes)
+    counts = (torch.empty if N else torch.zeros)((B,), dtype=torch.int32, device=target.device)
     lib = _lib.load()
     outs = (tokens.data_ptr(), path.data_ptr(), counts.data_ptr(), _lib.strides3(target))
     sizes = (B, N, V, _lib.TABLE_DTYPE_CODES[target.dtype])

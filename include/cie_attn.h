@@ -563,7 +563,7 @@ int cie_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_c
  *   tokens: like draft_tokens, the accepted nodes' tokens and the last one,
  *       then -1 (-1 as the last one where p has no positive entry)
  *   counts: int32 [B], the entries of path and tokens; 0 for a sequence whose
- *       node 0 is a padding slot
+ *       node 0 is a padding slot (N = 0: nothing is written, counts neither)
  * Only the rows of the visited nodes are read. cie_verify_greedy: a child is
  * accepted iff its token is the largest of target_logits at its parent (the
  * lowest index of equal ones, a NaN the largest), which is also the last token.
