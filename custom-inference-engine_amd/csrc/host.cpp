@@ -107,6 +107,12 @@ bool index_ok(const Tensor* t, const Tensor& like) {
 Tensor index32(const Tensor& t) {
   return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
 }
+// The same for operands whose values past 31 bits mean something (a marker below
+// every parent, an id or a length out of range): they stay on their side instead
+// of wrapping into the range.
+Tensor index32_clamped(const Tensor& t) {
+  return t.scalar_type() == at::kInt ? index32(t) : index32(t.clamp(INT32_MIN, INT32_MAX));
+}
 const int32_t* ip(const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
 
 struct Strides {
@@ -597,7 +603,7 @@ PyObject* masks(PyObject*, PyObject* const* a, Py_ssize_t n) {
                  (status->scalar_type() != at::kInt && status->scalar_type() != at::kUInt32)))
     Py_RETURN_NONE;
   const c10::OptionalDeviceGuard guard(p->device());
-  const Tensor par = index32(*p);
+  const Tensor par = index32_clamped(*p);
   const int64_t N = par.size(-1), B = par.dim() == 2 ? par.size(0) : 1;
   at::DimVector shape(par.sizes().begin(), par.sizes().end());
   const Tensor depths = at::empty(shape, par.options());
@@ -658,7 +664,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor out = o ? *o : at::empty({B, Hq, N, D}, q->options());
   const size_t nbytes = api.tree_ws((int)B, (int)Hq, (int)P.Hk, (int)N, (int)D, (int)mc, (int)P.block_size, (int)P.width);
   const Tensor ws = nbytes ? bytes_like(nbytes, *q) : Tensor();
-  const Tensor qc = laid_out(*q), bt = index32(*P.bt), lens = index32(*P.lens);
+  const Tensor qc = laid_out(*q), bt = index32_clamped(*P.bt), lens = index32_clamped(*P.lens);
   const Tensor kc = kn ? laid_out(*kn) : Tensor(), vc = kn ? laid_out(*vn) : Tensor();
   const Strides sq(qc), sk(*P.kc), sv(*P.vc), so(out), skn(kn ? kc : qc), svn(kn ? vc : qc);
   void* stream = stream_of(*q);
@@ -699,7 +705,7 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int replacement = PyObject_IsTrue(a[5]);
   if (replacement < 0) return nullptr;
   const c10::OptionalDeviceGuard guard(t->device());
-  const Tensor xc = x->contiguous(), pc = index32(*p), uc = u ? u->contiguous() : Tensor();
+  const Tensor xc = x->contiguous(), pc = index32_clamped(*p), uc = u ? u->contiguous() : Tensor();
   const Tensor tokens = at::empty({B, N}, xc.options()), path = at::empty({B, N}, pc.options());
   // (the library writes nothing for trees without nodes)
   const Tensor counts = N ? at::empty({B}, pc.options()) : at::zeros({B}, pc.options());
@@ -752,7 +758,8 @@ PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (bt->size(0) != B || pa->size(0) != B || cn->size(0) != B || !fits(B) || !fits(pa->size(1)) || !fits(bt->size(1)))
     Py_RETURN_NONE;
   const c10::OptionalDeviceGuard guard(first[0]->device());
-  const Tensor btc = index32(*bt), stc = index32(*st), pac = index32(*pa), cnc = index32(*cn);
+  const Tensor btc = index32_clamped(*bt), stc = index32_clamped(*st), pac = index32_clamped(*pa),
+               cnc = index32_clamped(*cn);
   void* stream = stream_of(*first[0]);
   const int rc = launch([&] {
     return api.keep(ptr[0].data(), ptr[1].data(), (int)layers, P.strides, P.strides + 3, ip(btc), ip(stc), ip(pac),

@@ -251,5 +251,14 @@ def strides3(t: torch.Tensor) -> ctypes.Array:
     return (ctypes.c_int64 * 3)(*st)
 
 
+def index32(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous int32 of ``t``; int64 values past 31 bits stay on their side
+    (a marker below every parent, an id or a length out of range) instead of
+    wrapping into the range."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(torch.int32).contiguous()
+
+
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream

@@ -641,8 +641,7 @@ def tree_attention(
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     lib = _lib.load()
-    bt = block_tables.to(torch.int32).contiguous()
-    lens = context_lens.to(torch.int32).contiguous()
+    bt, lens = _lib.index32(block_tables), _lib.index32(context_lens)
     mask = tree_mask if tree_mask.stride(-1) == 1 and tree_mask.stride(-2) == W else tree_mask.contiguous()
     if depths is not None and depths.stride(-1) != 1:
         depths = depths.contiguous()

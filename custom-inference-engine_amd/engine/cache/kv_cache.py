@@ -260,7 +260,7 @@ def kv_keep(k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor], 
         if t.stride(-1) != 1 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in range(3)):
             raise ValueError("kv_keep needs pools with a unit last stride, 16-byte aligned rows and outer strides in "
                              "multiples of 8 elements")
-    bt, st, pa, cn = (t.to(torch.int32).contiguous() for t in (block_tables, starts, path, counts))
+    bt, st, pa, cn = (_lib.index32(t) for t in (block_tables, starts, path, counts))
     n = len(k_caches)
     ptrs = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in pools]) for pools in (k_caches, v_caches)]
     byte_strides = [(ctypes.c_int64 * 3)(*[0 if t.shape[i] == 1 else 2 * t.stride(i) for i in range(3)])

@@ -75,7 +75,7 @@ def draft_tree(parents: torch.Tensor, status: torch.Tensor | None = None) -> Dra
     if status is not None and (not status.is_cuda or status.device != parents.device or status.numel() < 1
                                or status.dtype not in (torch.int32, torch.uint32)):
         raise ValueError("status must be an int32 tensor on parents' device")
-    p = parents.to(torch.int32).contiguous()
+    p = _lib.index32(parents)
     N = p.shape[-1]
     B = p.shape[0] if p.dim() == 2 else 1
     mask = torch.empty((*p.shape, -(-N // 32)), dtype=torch.int32, device=p.device)
@@ -120,7 +120,7 @@ def _verify(name: str, target: torch.Tensor, draft_tokens: torch.Tensor, parents
     if draft is not None and draft.stride(-1) != 1:
         draft = draft.contiguous()
     draft_tokens = draft_tokens.contiguous()
-    parents = parents.to(torch.int32).expand(B, N).contiguous()
+    parents = _lib.index32(parents).expand(B, N).contiguous()
     tokens = torch.empty_like(draft_tokens)
     path = torch.empty_like(parents)
     # (the library writes nothing for trees without nodes)
