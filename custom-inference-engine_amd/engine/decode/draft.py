@@ -167,8 +167,9 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, parents
     ``max(p - q, 0)`` and, without replacement, q loses x, each over its sum
     (unless that is below 2^-40). With picks q(x) is 1 and p loses x. When no
     child is accepted, the last token is the first y at which the running sum of
-    p exceeds ``u_0 sum(p)``. All of it is computed in 64 bits, from the rows of
-    the visited nodes alone; nothing waits for the GPU."""
+    p exceeds ``u_0 sum(p)``. All of it is computed in 64 bits. The rows of the
+    visited nodes alone decide, but entries of all others are read too: nothing
+    else may write them meanwhile. Nothing waits for the GPU."""
     if uniforms is None:
         raise ValueError("verify_draft needs uniforms; verify_greedy takes none")
     return _verify("verify_draft", target_probs, draft_tokens, parents, uniforms, draft_probs, bool(replacement))

@@ -564,9 +564,12 @@ int cie_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_c
  *       then -1 (-1 as the last one where p has no positive entry)
  *   counts: int32 [B], the entries of path and tokens; 0 for a sequence whose
  *       node 0 is a padding slot (N = 0: nothing is written, counts neither)
- * Only the rows of the visited nodes are read. cie_verify_greedy: a child is
- * accepted iff its token is the largest of target_logits at its parent (the
- * lowest index of equal ones, a NaN the largest), which is also the last token.
+ * The rows of the visited nodes alone decide, but all B x N rows of target_probs
+ * and draft_probs must be readable: single entries of every parent's row are
+ * fetched before the walk, and cie_verify_greedy with a workspace reads every row
+ * whole. cie_verify_greedy: a child is accepted iff its token is the largest of
+ * target_logits at its parent (the lowest index of equal ones, a NaN the
+ * largest), which is also the last token.
  * Its workspace: cie_verify_greedy_workspace_bytes bytes, 16-byte aligned, any
  * contents, not shared by concurrent calls; 0 bytes (NULL allowed) when the rows
  * are to be read one after another as the walk comes to them, which is chosen

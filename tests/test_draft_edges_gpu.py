@@ -8,6 +8,7 @@ import torch
 from engine.attention import tree_attention
 from engine.cache import kv_keep
 from engine.decode import draft_tree, verify_draft, verify_greedy
+from test_draft_gpu import make
 from test_tree_gpu import Case
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +82,28 @@ def test_int64_ids_and_lengths_out_of_range_are_nan():
         n[1] += 2 ** 32
         out = tree_attention(q, k, v, ids, n, m)
         assert torch.isnan(out[:2].float()).all() and torch.equal(out[2], clean[2])
+
+
+@pytest.mark.parametrize("mode,V", [("greedy", 501), ("greedy", 1_500_000), ("picks", 501), ("iid", 501), ("tree", 501)])
+def test_rows_that_no_walk_visits_decide_nothing(mode, V):
+    # (the larger vocabulary is over 64 MiB of logits: its rows are read on the walk)
+    B, N, dtype = 3, 14, torch.bfloat16 if V > 501 else torch.float32
+    target, tokens, parents, u, draft = make(B, N, 501, dtype, mode, seed=7)
+    parents = [p[:12] + [-2, -2] for p in parents]
+    t, x, p = target.to(DEV), dev(tokens, torch.int64), dev(parents)
+    if V > 501:
+        wide = torch.full((B, N, V), -50.0, dtype=dtype, device=DEV)
+        wide[..., :501] = t
+        t = wide
+    d = None if draft is None else draft.to(DEV)
+    run = lambda: (verify_greedy(t, x, p) if mode == "greedy" else  # noqa: E731
+                   verify_draft(t, x, p, dev(u, torch.float32), d, replacement=mode == "iid"))
+    want = run()
+    unseen = torch.ones((B, N), dtype=torch.bool, device=DEV)
+    for b, n in enumerate(want.counts.tolist()):
+        unseen[b, want.path[b, :n].long()] = False
+    for bad in (float("nan"), float("inf")):
+        for rows in (t, d):
+            if rows is not None:
+                rows[unseen] = bad
+        assert all(torch.equal(a, b) for a, b in zip(run(), want))
