@@ -284,6 +284,7 @@ def prepare(c, seed):
     if c["kind"] == "keep":
         shape = (c["layers"], blocks, BS, Hk, D)
         s["k"], s["v"] = _randn(g, *shape, dtype=dtype), _randn(g, *shape, dtype=dtype)
+        s["pools"] = [list(s[x].unbind(0)) for x in "kv"]  # a cache holds its layers' pools as lists
         paths = _kept(c)
         s["path"] = torch.tensor([p + [-1] * (N - len(p)) for p in paths], dtype=torch.int32).to(DEV)
         s["counts"] = torch.tensor([len(p) for p in paths], dtype=torch.int32).to(DEV)
@@ -328,8 +329,7 @@ def run(s):
                     r = e.decode.verify_draft(s["target"], s["tokens"], s["parents"], s["u"],
                                               draft_probs=s.get("draft"), replacement=c["mode"] == "iid")
                 return r.tokens, r.path, r.counts
-            e.cache.kv_keep(list(s["k"].unbind(0)), list(s["v"].unbind(0)), s["bt"], s["starts"], s["path"],
-                            s["counts"])
+            e.cache.kv_keep(*s["pools"], s["bt"], s["starts"], s["path"], s["counts"])
             return s["k"], s["v"]
         if c["kind"] == "attend":
             return _plain_attend(s, _plain_bits(s["mask"], c["N"]))
