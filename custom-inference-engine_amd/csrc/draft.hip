@@ -14,9 +14,11 @@ namespace cie {
 //
 // One workgroup per sequence, one thread per node. A parent's index is below
 // its child's, so the walk to the root meets the ancestors in falling order:
-// the row's words are finished one after another, and every walk ends. The
-// work is N dependent LDS reads at most (a chain); 1 x 8 nodes 1.7-1.9 us, the
-// time of an empty launch, 8 x 26 2.7-4.8.
+// the row's words are finished one after another, and every walk ends. A thread
+// walks twice, for the depth and validity and for the bits: two dependent LDS reads
+// a level of the tree, 0.19 us. Trees of a few levels 1.7-1.9 us up to 128 nodes,
+// the time of an empty launch, and 5 and 18 for 512 and 1024 nodes, whose threads
+// each write a row of their own; a chain of 26 nodes 5.3, of 128 23, of 1024 194.
 __global__ __launch_bounds__(1024) void draft_mask_kernel(const int32_t* parents, int32_t* mask, int32_t* depths,
                                                          uint32_t* status, int N, int W) {
   __shared__ int32_t par[kTreeMaxNodes];
@@ -91,11 +93,16 @@ hipError_t launch_draft_masks(const int32_t* parents, int32_t* mask, int32_t* de
 // part holding the last token follows from them and only it is read again.
 //
 // One workgroup per sequence: start 1-1.5 us, a step down the tree 0.1, the last
-// token 2.8, and the passes, at what one CU reads (wave_sums). 8 chains of 5 over
-// 32000 fp32 tokens 8-10 us, most of it one pass of p; 32 trees of 26 over 128000
-// 44-57, the sequence with three rejections at a node. (Summing every row with the
-// whole GPU beforehand, for c = 1: 63 -> 150 us there, 16.6 -> 20 for the chains:
-// the walk needs few of them.)
+// token 2.8, and the passes, at what one CU reads (wave_sums), one after another and
+// with the other CUs idle where sequences are few. Over 128000 fp32 tokens a call
+// without a rejection takes 11 us whatever the batch; each rejection adds 10 (with
+// replacement) or 13 (without), the first one some 10 more for a draft's own picks
+// and 2 for every other: one sequence with eight rejections at a node 97, 127 and 34.
+// 8 chains of 5 over 32000 tokens 8-10 us, most of it one pass of p; 32 trees of 26
+// over 128000 44-57, the sequence with three rejections at a node. (Summing every row
+// with the whole GPU beforehand, for c = 1: 63 -> 150 us there, 16.6 -> 20 for the
+// chains: the walk needs few of them. Only the rows of nodes whose first child fails
+// are needed, which the gathered p, q and u tell; not built.)
 constexpr int kVerifyWaves = 16, kVerifyThreads = 64 * kVerifyWaves;
 constexpr int kParts = 64;
 constexpr double kNoMass = 0x1p-40;
@@ -681,11 +688,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_greedy_kernel(const Ver
 
 // All rows first or one after another on the walk? The first costs the bytes of
 // the logits at 4.3 TB/s and a launch, whatever is accepted; the second 3 to 5 us
-// a visited node, whose row one CU reads at some 80 GB/s. Measured, bf16 (us,
-// rows first / on the walk, 2 to 5 nodes visited): 128000 tokens, 1 x 26
-// 12.9 / 25.2, 8 x 26 16.9 / 26.7, 16 x 26 (106 MB) 26.5 / 28.2, 32 x 26
+// a visited node of 128000 tokens, whose row one CU reads at some 80 GB/s, for the
+// sequence that accepts most. All rows first while they are 64 MiB at most. Measured,
+// bf16 (us, rows first / on the walk, 2 to 5 nodes visited): 128000 tokens, 1 x 26
+// 12.9 / 25.2, 8 x 26 (53 MB) 16.9 / 26.7, 16 x 26 (106 MB) 26.5 / 25.6-28.2, 32 x 26
 // 46.0 / 28.8; 32000 tokens, 1 x 8 12.5 / 13.2, 64 x 8 (33 MB) 13.9 / 16.3,
-// 64 x 26 (106 MB) 26.9 / 20.2.
+// 64 x 26 (106 MB) 26.9 / 20.2. Where the two meet depends on the nodes visited, which
+// the host does not know: at 106 MB of the larger vocabulary they are equal, and a
+// batch of few, deep paths would gain from rows first there.
 size_t verify_tops_bytes(int B, int N, int V, int dtype) {
   const int64_t rows = (int64_t)B * N;
   if (rows > (64ll << 20) / ((int64_t)V * (dtype == 2 ? 4 : 2)) || rows > 1 << 20) return 0;  // (and one launch)

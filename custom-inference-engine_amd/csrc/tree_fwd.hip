@@ -127,9 +127,13 @@ __device__ __forceinline__ int tree_position(int base, int depth) {
   return (int)min((uint32_t)base + (uint32_t)max(depth, 0), 0x7fffffffu);
 }
 
+// Waits for a tile, `ahead` tiles having been issued after it, of PT copies each
+// (vmcnt counts them). It leaves three of those outstanding at most: with a ring of
+// more than six stages (seven for QT = 8) a step also waits for tiles that it does not
+// need yet, and at D = 256 with QT = 1, whose PT is 32, the first wait is for all tiles
+// issued.
 template <int PT>
 __device__ __forceinline__ void tree_wait(int ahead) {
-  // vmcnt counts the PT copies of every tile issued after the one needed
   if constexpr (3 * PT < 64) {
     if (ahead >= 3) { vm_wait<3 * PT>(); return; }
   }
@@ -683,7 +687,7 @@ TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int b
   // with two workgroups of 64 KiB and stages of 32 and 16.
   g.NST = std::min(8, std::max(3, (int)((size_t)128 * 1024 / stage)));
   const int cpt = 2 * (D / (16 * std::min(g.QT, D / 16)));  // copies of an issuing wave per tile
-  g.NST = std::min(g.NST, 3 + 63 / cpt);                    // those of NST - 3 tiles in flight fit vmcnt
+  g.NST = std::min(g.NST, 3 + 63 / cpt);                    // copies of NST - 3 tiles fit vmcnt (see tree_wait)
   // nor more stages than the longest sequence has tiles (and those that reach leaves
   // free): short ones then share a CU
   const int64_t most = (ctx_limit + kPagedTile - 1) / kPagedTile + (g.QT == 8 ? 2 : 1);
@@ -696,17 +700,21 @@ TreeGeom tree_geometry(int B, int Hq, int Hk, int N, int D, int ctx_limit, int b
   const int64_t nt_max = (int64_t)B * ((ctx_limit + kPagedTile - 1) / kPagedTile);
   // tiles whose block ids the workgroup can stage
   const int64_t ccap = std::max<int64_t>(1, ((int64_t)(kTreeIds - 2) * block_size) / kPagedTile);
-  // Pieces beyond one per sequence. While the sequences' workgroups take at most half
-  // of the CUs: what fills them once, one workgroup per CU, in pieces of two tiles at
-  // least (one tile: 1 x 8 nodes over 777 tokens 12.0 -> 12.3 us; four: 13.5). Above
-  // that a piece has to pay for its start, the time of some six tiles, and for its
-  // partial states: only sequences of more than the average are cut, and of more than
-  // 32 tiles while every workgroup has a CU (10 of 11 nodes over 132-2112 tokens 50 us,
-  // of more than 64 tiles 68, than 8 51; 20 of 64 over 700-800 39.6, 39.0, 54.0), 64
-  // when they come in rounds (48 of 26 over 1000-2000 58, than 32 70). Against two to
-  // four pieces of two tiles or more per sequence: 41 of 110 over 33 tokens 68 -> 30,
-  // 22 of 64 over 900 87 -> 42, 17 of 200 over 300-4000 378 -> 256, 48 of 8 over 4000
-  // 158 -> 133; but 33 of 16 over 500-8000 108 -> 119, 48 of 26 over 2000-4000 126 -> 134.
+  // Pieces beyond one per sequence, by W = B * per_piece, the workgroups of whole
+  // sequences:
+  //   2 W <= CUs: as many as fill the CUs once, one workgroup each, of two tiles at least
+  //     (1 x 8 nodes over 777 tokens 12.0 us; of one tile 12.3, of four 13.5);
+  //   above: as many as there are sequences, so that only those of more tiles than the
+  //     average are cut, as a piece pays for its start, the time of some six tiles, and
+  //     for its partial states; and none of 32 tiles or fewer while every workgroup has a
+  //     CU (10 of 11 nodes over 132-2112 tokens 50 us; none of 64 68, of 8 51), of 64
+  //     when they come in rounds (48 of 26 over 1000-2000 58; of 32 70).
+  // Against two to four pieces of two tiles or more for every sequence the second rule
+  // wins much where sequences are short or rows are many (41 of 110 over 33 tokens
+  // 68 -> 30, 22 of 64 over 900 87 -> 42, 17 of 200 over 300-4000 378 -> 256, 48 of 8 over
+  // 4000 158 -> 133) and loses a little where few rows read long ragged histories (33
+  // of 16 over 500-8000 108 -> 119, 48 of 26 over 2000-4000 126 -> 134). All with P in one
+  // part, as the ring's figures above.
   const int64_t per_piece = (int64_t)g.NG * g.NRT;
   const bool busy = 2 * B * per_piece > dev.cus;
   int64_t extra = busy ? B : std::max<int64_t>(1, dev.cus / per_piece - B);
