@@ -77,7 +77,8 @@ def tree_attention_f64(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, see: t
             reach = float((kk.abs() @ qq.abs()).max()) * abs(scale)  # sum of |products| behind a score
             eps32 = 2.0 ** -24 * (2 * (D + 8) * reach + parts * L + 64)
             # probabilities are rounded relative to the running maximum, the largest being up to 1
-            bound[hq, i] = h * out[hq, i].abs() + h ** parts * a * (1 + h) + tiny * (1 + top * vv.abs().sum(0)) + eps32 * a
+            bound[hq, i] = (h * out[hq, i].abs() + h ** parts * a * (1 + h) + tiny * (1 + top * vv.abs().sum(0))
+                            + eps32 * a)
     return out, bound
 
 
